@@ -23,9 +23,10 @@ EXPORTED_SYMBOLS = (
     "fcs_statistics_rows", "fcs_colsum_statistics", "fcs_colsum_columns", "fcs_selftest_wait_expiry",
     "fcs_selftest_wait_expiry_cluster",
     "fcs_peer_post", "fcs_peer_wait", "fcs_colsum_causal_accumulate_signalled",
+    "fcs_append_paged", "fcs_select_pages", "fcs_select_pages_workspace_bytes", "fcs_attend_pages",
 )
 
-ABI_VERSION = 202   # fcs_version() of the library these argument lists were written for
+ABI_VERSION = 203   # fcs_version() of the library these argument lists were written for
 FCS_OK = 0
 FCS_ERR_UNSUPPORTED = -2
 FCS_DTYPE_FP16 = 0
@@ -41,6 +42,23 @@ class PeerSignals(ctypes.Structure):
     """`FcsPeerSignals` of the header."""
     _fields_ = [("wait_flag", _p), ("wait_value", _i), ("post", _p * 15), ("post_n", _i), ("post_value", _i),
                 ("counter", _p), ("done_flag", _p), ("done_value", _i)]
+
+
+class PagedCache(ctypes.Structure):
+    """`FcsPagedCache` of the header."""
+    _fields_ = [("key_pages", _p), ("value_pages", _p), ("key_stride", _i64 * 3), ("value_stride", _i64 * 3),
+                ("page_table", _p), ("table_stride", _i64), ("lens", _p), ("starts", _p),
+                ("pages", _i), ("kv_heads", _i), ("page_size", _i), ("dim", _i), ("dtype", _i),
+                ("sequences", _i), ("table_width", _i), ("tokens", _i)]
+
+
+class PagedRows(ctypes.Structure):
+    """`FcsPagedRows` of the header."""
+    _fields_ = [("key", _p), ("value", _p), ("query", _p), ("query_out", _p),
+                ("key_stride", _i64 * 2), ("value_stride", _i64 * 2), ("query_stride", _i64 * 2),
+                ("query_out_stride", _i64 * 2), ("q_heads", _i), ("cos", _p), ("sin", _p),
+                ("table_rows", _i), ("rotary", _i), ("interleaved", _i), ("positions", _p), ("bounds", _p),
+                ("fill_tail", _i)]
 
 
 class LibraryMissing(RuntimeError):
@@ -127,6 +145,15 @@ def load() -> ctypes.CDLL:
     lib.fcs_colsum_batched_static_scratch.restype = _i
     lib.fcs_colsum_batched_static_scratch.argtypes = [_p, _p, _p, _i64, _i, _i, _i, _i, _i] + [_i64] * 6 + \
         [_f, _i, _i, _p, _p]
+    cache = ctypes.POINTER(PagedCache)
+    lib.fcs_append_paged.restype = _i
+    lib.fcs_append_paged.argtypes = [cache, ctypes.POINTER(PagedRows), _p, _p]
+    lib.fcs_select_pages_workspace_bytes.restype = _sz
+    lib.fcs_select_pages_workspace_bytes.argtypes = [cache]
+    lib.fcs_select_pages.restype = _i
+    lib.fcs_select_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _i, _i, _p, _i, _p, _sz, _p, _p]
+    lib.fcs_attend_pages.restype = _i
+    lib.fcs_attend_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _f, _p, ctypes.POINTER(_i64), _p, _i, _p, _p]
     lib.fcs_set_profiling.restype = _i
     lib.fcs_set_profiling.argtypes = [_i]
     lib.fcs_set_single_pass.restype = _i

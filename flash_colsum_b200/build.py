@@ -9,6 +9,7 @@ so this works on a machine without a GPU.
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -19,23 +20,32 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflash_colsum_b200.so")
-SOURCES = [os.path.join(CSRC, "flash_colsum_sm100.cu")]
-HEADERS = [os.path.join(CSRC, "sm100_ptx.cuh"), os.path.join(CSRC, "schedule.h"),
-           os.path.join(CSRC, "colsum_small_q.cuh"), os.path.join(CSRC, "colsum_few_rows.cuh"),
-           os.path.join(CSRC, "round_fp32.cuh"), os.path.join(CSRC, "colsum_math.cuh"),
-           os.path.join(CSRC, "colsum_single_pass.cuh"), os.path.join(CSRC, "select_topk.cuh"),
-           os.path.join(CSRC, "colsum_fused_short.cuh"), os.path.join(CSRC, "host_api.h"),
-           os.path.join(os.path.dirname(PKG), "include", "flash_colsum_b200.h")]
+_ABI = os.path.join(os.path.dirname(PKG), "include", "flash_colsum_b200.h")
+
+
+def _csrc(*names):
+    return [os.path.join(CSRC, name) for name in names]
+
+
+# The library's translation units and the headers each is compiled from.
+UNITS = {
+    _csrc("flash_colsum_sm100.cu")[0]: _csrc(
+        "sm100_ptx.cuh", "schedule.h", "colsum_small_q.cuh", "colsum_few_rows.cuh", "round_fp32.cuh", "colsum_math.cuh",
+        "colsum_single_pass.cuh", "select_topk.cuh", "colsum_fused_short.cuh", "host_api.h", "host_common.h") + [_ABI],
+    _csrc("paged_sm100.cu")[0]: _csrc(
+        "sm100_ptx.cuh", "paged.cuh", "paged_append.cuh", "paged_select.cuh", "paged_attend.cuh",
+        "host_common.h") + [_ABI],
+}
+SOURCES = list(UNITS)
+HEADERS = sorted({header for headers in UNITS.values() for header in headers})
 
 # the operator's host path for PyTorch callers: a CPython extension module over the library above
 BINDING_NAME = "_fcs_torch"
 BINDING_PATH = os.path.join(LIB_DIR, BINDING_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
-BINDING_HEADERS = [os.path.join(CSRC, "host_api.h"),
-                   os.path.join(os.path.dirname(PKG), "include", "flash_colsum_b200.h")]
+BINDING_HEADERS = _csrc("host_api.h") + [_ABI]
 
-NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC"]
+NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 
 def find_nvcc() -> str:
@@ -69,8 +79,18 @@ def _compile(cmd, target: str, verbose: bool) -> None:
         print(res.stderr)
 
 
-def _build_library(verbose: bool) -> None:
-    _compile([find_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + SOURCES, LIB_PATH, verbose)
+def _object(source: str) -> str:
+    return os.path.join(LIB_DIR, os.path.splitext(os.path.basename(source))[0] + ".o")
+
+
+def _build_library(force: bool, verbose: bool) -> None:
+    """Compile the units that are older than their sources, at the same time, and link the library."""
+    nvcc = [find_nvcc()] + NVCC_FLAGS
+    flags = ["-Xptxas", "-v"] if verbose else []
+    stale = [unit for unit, headers in UNITS.items() if force or _older(_object(unit), [unit] + headers)]
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        list(pool.map(lambda unit: _compile(nvcc + flags + ["-c", unit], _object(unit), verbose), stale))
+    _compile(nvcc + ["-shared"] + [_object(unit) for unit in UNITS], LIB_PATH, False)
 
 
 def _build_binding(verbose: bool) -> None:
@@ -99,7 +119,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
             if force or _older(LIB_PATH, SOURCES + HEADERS):
-                _build_library(verbose)
+                _build_library(force, verbose)
             if force or _older(BINDING_PATH, [BINDING_SOURCE] + BINDING_HEADERS):
                 _build_binding(verbose)
         finally:

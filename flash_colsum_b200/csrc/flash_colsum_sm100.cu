@@ -47,6 +47,7 @@
 
 #include "../../include/flash_colsum_b200.h"
 #include "host_api.h"
+#include "host_common.h"
 
 #include "colsum_single_pass.cuh"
 #include "select_topk.cuh"
@@ -888,9 +889,9 @@ __global__ void peer_wait_kernel(const int* flags, int n, int value, int* status
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-static thread_local char g_err[512] = "";
+thread_local char g_err[512] = "";
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -898,12 +899,7 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
+EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         void* sym = nullptr;
@@ -915,7 +911,7 @@ static EncodeTiledFn encode_tiled_fn() {
     return fn;
 }
 
-static int num_sms() {
+int num_sms() {
     static int cached[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
@@ -931,7 +927,7 @@ static int num_sms() {
 // elements, 128-byte swizzle, out-of-range rows read as zero -- and so do the columns
 // from D on when D is not a multiple of 64: the kernels contract 64 or 128 columns, the
 // padding adds nothing to a score.
-static int make_tensor_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int S, int D,
+int make_tensor_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int S, int D,
                            int64_t sb, int64_t sh, int64_t ss, int box_rows) {
     EncodeTiledFn enc = encode_tiled_fn();
     if (!enc) return fail(FCS_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
@@ -2185,7 +2181,7 @@ static int static_scratch_address(void** out_ptr) {
 // ---------------------------------------------------------------------------
 extern "C" {
 
-int fcs_version(void) { return 202; }
+int fcs_version(void) { return 203; }
 
 const char* fcs_last_error(void) { return fcs::g_err; }
 

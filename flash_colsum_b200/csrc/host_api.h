@@ -46,6 +46,12 @@ typedef int (*FcsRunHostCallFn)(const FcsHostCall*);
 typedef int (*FcsSelectTopkFn)(const float*, int64_t, int, int, int, int*, float*, void*);
 typedef int (*FcsSelectThresholdFn)(const float*, int64_t, int, int, float, int, int*, int*, void*);
 typedef const char* (*FcsLastErrorFn)(void);
+typedef int (*FcsAppendPagedFn)(const FcsPagedCache*, const FcsPagedRows*, int*, void*);
+typedef size_t (*FcsSelectPagesWorkspaceFn)(const FcsPagedCache*);
+typedef int (*FcsSelectPagesFn)(const FcsPagedCache*, const void*, const int64_t*, int, const void*, int, int, int, int*, int,
+                                void*, size_t, int*, void*);
+typedef int (*FcsAttendPagesFn)(const FcsPagedCache*, const void*, const int64_t*, int, const int*, int, float, void*,
+                                const int64_t*, float*, int, int*, void*);
 
 int fcs_run_call(const FcsCall* call);
 

@@ -1,0 +1,332 @@
+// Entry points over a paged cache: appending to it, choosing pages of it, attending over chosen pages.  The kernels are in
+// paged_append.cuh, paged_select.cuh and paged_attend.cuh.
+#include <float.h>
+#include <math.h>
+#include <string.h>
+
+#include "../../include/flash_colsum_b200.h"
+#include "host_common.h"
+#include "paged_append.cuh"
+#include "paged_select.cuh"
+#include "paged_attend.cuh"
+
+namespace fcs {
+namespace paged {
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Strides (in elements) of `n` outer axes of a tensor of 16-bit elements whose rows are read in pieces of 16 bytes.
+static int check_rows(const char* name, const void* ptr, const int64_t* stride, int n) {
+    if (!ptr) return fail(FCS_ERR_INVALID_ARGUMENT, "%s is NULL", name);
+    if (!aligned16(ptr)) return fail(FCS_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned", name);
+    for (int i = 0; i < n; ++i)
+        if (stride[i] < 0 || stride[i] % 8)
+            return fail(FCS_ERR_INVALID_ARGUMENT, "%s strides must not be negative and be multiples of 8 elements", name);
+    return FCS_OK;
+}
+
+static int check_cache(const FcsPagedCache* c, Batch& out, int* status) {
+    if (!c) return fail(FCS_ERR_INVALID_ARGUMENT, "cache is NULL");
+    if (c->dim % 8 || c->dim < 8 || c->dim > 128)
+        return fail(FCS_ERR_UNSUPPORTED, "head dimension must be a multiple of 8 from 8 to 128, got %d", c->dim);
+    if (c->dtype != FCS_DTYPE_FP16 && c->dtype != FCS_DTYPE_BF16)
+        return fail(FCS_ERR_UNSUPPORTED, "dtype must be FCS_DTYPE_FP16 or FCS_DTYPE_BF16, got %d", c->dtype);
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+        return fail(FCS_ERR_UNSUPPORTED, "page size must be 16, 32, 64 or 128, got %d", c->page_size);
+    if (c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 || c->sequences <= 0 || c->table_width <= 0 || c->tokens <= 0)
+        return fail(FCS_ERR_INVALID_ARGUMENT, "sizes must be positive (pages=%d kv_heads=%d sequences=%d table_width=%d tokens=%d)",
+                    c->pages, c->kv_heads, c->sequences, c->table_width, c->tokens);
+    if (!c->page_table || !c->lens) return fail(FCS_ERR_INVALID_ARGUMENT, "page_table and lens must not be NULL");
+    if (c->table_stride < c->table_width && c->sequences > 1)
+        return fail(FCS_ERR_INVALID_ARGUMENT, "table_stride (%lld) is smaller than the table's width", (long long)c->table_stride);
+    if (!c->starts && c->tokens != c->sequences)
+        return fail(FCS_ERR_INVALID_ARGUMENT, "without starts there is one token a sequence, got %d tokens and %d sequences",
+                    c->tokens, c->sequences);
+    out.table = c->page_table;
+    out.table_ld = c->table_stride;
+    out.lens = c->lens;
+    out.starts = c->starts;
+    out.pages = c->pages;
+    out.kv_heads = c->kv_heads;
+    out.page_shift = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+    out.dim = c->dim;
+    out.sequences = c->sequences;
+    out.width = c->table_width;
+    out.tokens = c->tokens;
+    out.status = status;
+    return FCS_OK;
+}
+
+static int check_group(const FcsPagedCache* c, int q_heads) {
+    if (q_heads <= 0 || q_heads % c->kv_heads)
+        return fail(FCS_ERR_INVALID_ARGUMENT, "query heads (%d) must be a multiple of the key heads (%d)", q_heads, c->kv_heads);
+    return FCS_OK;
+}
+
+// Every kernel may start while the one before it in the stream drains (it waits for it before it reads).
+template <typename... Params, typename... Args>
+static cudaError_t launch(void (*kern)(Params...), dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
+                          const Args&... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// ------------------------------------------------------------------ append
+static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status, cudaStream_t stream) {
+    AppendParams p;
+    memset(&p, 0, sizeof(p));
+    int rc = check_cache(cache, p.c, status);
+    if (rc != FCS_OK) return rc;
+    if (!r) return fail(FCS_ERR_INVALID_ARGUMENT, "rows is NULL");
+    if ((rc = check_rows("key", r->key, r->key_stride, 2)) != FCS_OK) return rc;
+    if ((rc = check_rows("value", r->value, r->value_stride, 2)) != FCS_OK) return rc;
+    if ((rc = check_rows("key_pages", cache->key_pages, cache->key_stride, 3)) != FCS_OK) return rc;
+    if ((rc = check_rows("value_pages", cache->value_pages, cache->value_stride, 3)) != FCS_OK) return rc;
+    const bool with_query = r->query != nullptr;
+    if (with_query) {
+        if ((rc = check_rows("query", r->query, r->query_stride, 2)) != FCS_OK) return rc;
+        if ((rc = check_rows("query_out", r->query_out, r->query_out_stride, 2)) != FCS_OK) return rc;
+        if ((rc = check_group(cache, r->q_heads)) != FCS_OK) return rc;
+        if (r->q_heads > 65535 * 8) return fail(FCS_ERR_UNSUPPORTED, "too many query heads (%d)", r->q_heads);
+    }
+    if ((r->cos == nullptr) != (r->sin == nullptr)) return fail(FCS_ERR_INVALID_ARGUMENT, "cos and sin go together");
+    if (r->cos) {
+        if (!aligned16(r->cos) || !aligned16(r->sin)) return fail(FCS_ERR_INVALID_ARGUMENT, "cos and sin must be 16-byte aligned");
+        if (r->rotary % 16 || r->rotary < 16 || r->rotary > cache->dim)
+            return fail(FCS_ERR_UNSUPPORTED, "the rotated features must be a multiple of 16 up to the head dimension, got %d", r->rotary);
+        if (r->table_rows <= 0) return fail(FCS_ERR_INVALID_ARGUMENT, "cos and sin have no rows");
+        p.cos = r->cos;
+        p.sin = r->sin;
+        p.rotary = r->rotary;
+        p.interleaved = r->interleaved != 0;
+        p.table_rows = r->table_rows;
+        p.positions = r->positions;
+    }
+    if (r->bounds && !aligned16(r->bounds)) return fail(FCS_ERR_INVALID_ARGUMENT, "bounds must be 16-byte aligned");
+    p.key = static_cast<const uint16_t*>(r->key);
+    p.value = static_cast<const uint16_t*>(r->value);
+    p.query = static_cast<const uint16_t*>(r->query);
+    p.query_out = static_cast<uint16_t*>(r->query_out);
+    p.bounds = static_cast<uint16_t*>(r->bounds);
+    p.key_pages = static_cast<uint16_t*>(cache->key_pages);
+    p.value_pages = static_cast<uint16_t*>(cache->value_pages);
+    for (int i = 0; i < 2; ++i) {
+        p.key_st[i] = r->key_stride[i];
+        p.value_st[i] = r->value_stride[i];
+        p.query_st[i] = r->query_stride[i];
+        p.query_out_st[i] = r->query_out_stride[i];
+    }
+    for (int i = 0; i < 3; ++i) {
+        p.key_page_st[i] = cache->key_stride[i];
+        p.value_page_st[i] = cache->value_stride[i];
+    }
+    p.q_heads = with_query ? r->q_heads : 0;
+    p.fill_tail = r->fill_tail != 0;
+    // a CTA's rows: the heads of a group times the tokens of a page, about 64
+    const long long B = cache->sequences, T = cache->tokens, P = cache->page_size;
+    const long long each = cache->starts ? (T / B < P ? (T + B - 1) / B : P) : 1;
+    while (p.heads_shift < 4 && (each << p.heads_shift) < 64) ++p.heads_shift;
+    const int heads = 1 << p.heads_shift;
+    p.kv_groups = (cache->kv_heads + heads - 1) / heads;
+    const long long segments = cache->starts ? T / P + 2 * B + 1 : B;
+    const long long groups = 2ll * p.kv_groups + (p.q_heads + heads - 1) / heads;
+    if (segments > 0x7fffffffll || groups > 65535)
+        return fail(FCS_ERR_UNSUPPORTED, "the call is too large for one launch (%lld tokens, %d heads)", T, p.q_heads);
+    const dim3 grid((unsigned)segments, (unsigned)groups);
+    const cudaError_t e = cache->dtype == FCS_DTYPE_BF16
+                              ? launch(append_kernel<Bf16Ops>, grid, APPEND_THREADS, 0, 1, stream, p)
+                              : launch(append_kernel<HalfOps>, grid, APPEND_THREADS, 0, 1, stream, p);
+    if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "appending failed to launch: %s", cudaGetErrorString(e));
+    return FCS_OK;
+}
+
+// ------------------------------------------------------------------ select
+// Tokens whose scores are held at once: 256 MiB of them, and as many as a grid takes.
+static long long select_tokens_at_once(const FcsPagedCache* c) {
+    const long long row = 8ll * c->kv_heads * c->table_width;
+    long long n = (256ll << 20) / row;
+    n = n < 1 ? 1 : n > 32768 ? 32768 : n;
+    return n < c->tokens ? n : c->tokens;
+}
+
+static size_t select_workspace(const FcsPagedCache* c) {
+    return (size_t)select_tokens_at_once(c) * c->kv_heads * c->table_width * 8;
+}
+
+static int select(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const void* bounds,
+                  int k, int first, int last, int* chosen, int fill_tail, void* workspace, size_t workspace_bytes, int* status,
+                  cudaStream_t stream) {
+    SelectParams p;
+    memset(&p, 0, sizeof(p));
+    int rc = check_cache(cache, p.c, status);
+    if (rc != FCS_OK) return rc;
+    if (!query_stride) return fail(FCS_ERR_INVALID_ARGUMENT, "query strides are NULL");
+    if ((rc = check_rows("query", query, query_stride, 2)) != FCS_OK) return rc;
+    if ((rc = check_group(cache, q_heads)) != FCS_OK) return rc;
+    if (!bounds || !aligned16(bounds)) return fail(FCS_ERR_INVALID_ARGUMENT, "bounds must be a 16-byte aligned device pointer");
+    if (!chosen) return fail(FCS_ERR_INVALID_ARGUMENT, "chosen is NULL");
+    if (k < 1 || first < 0 || last < 1 || (long long)first + last > k)
+        return fail(FCS_ERR_INVALID_ARGUMENT, "k must hold the first and the last pages (k=%d first=%d last=%d)", k, first, last);
+    const size_t need = select_workspace(cache);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)
+        return fail(FCS_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes, got %zu", need, workspace_bytes);
+    p.query = static_cast<const uint16_t*>(query);
+    p.bounds = static_cast<const uint16_t*>(bounds);
+    p.query_st[0] = query_stride[0];
+    p.query_st[1] = query_stride[1];
+    p.group = q_heads / cache->kv_heads;
+    p.k = k;
+    p.first = first;
+    p.last = last;
+    p.chosen = chosen;
+    p.scores = static_cast<double*>(workspace);
+    p.fill_tail = fill_tail;
+    const long long at_once = select_tokens_at_once(cache);
+    for (long long t0 = 0; t0 < cache->tokens; t0 += at_once) {
+        const unsigned n = (unsigned)(cache->tokens - t0 < at_once ? cache->tokens - t0 : at_once);
+        p.t0 = (int)t0;
+        const dim3 grid((cache->table_width + SCORE_PAGES - 1) / SCORE_PAGES, cache->kv_heads, n);
+        cudaError_t e = cache->dtype == FCS_DTYPE_BF16 ? launch(score_kernel<true>, grid, SCORE_THREADS, 0, 1, stream, p)
+                                                       : launch(score_kernel<false>, grid, SCORE_THREADS, 0, 1, stream, p);
+        if (e == cudaSuccess) e = launch(choose_kernel, dim3(cache->kv_heads, n), CHOOSE_THREADS, 0, 1, stream, p);
+        if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "choosing pages failed to launch: %s", cudaGetErrorString(e));
+    }
+    return FCS_OK;
+}
+
+// ------------------------------------------------------------------ attend
+template <int DP, int NT, bool BF16, int CL>
+static cudaError_t launch_attend(const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t stream) {
+    constexpr int STAGES = DP == 128 ? 3 : 4;
+    using L = AttendLayout<DP, STAGES>;
+    auto* kern = attend_kernel<DP, NT, STAGES, BF16, CL>;
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !configured[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) configured[dev] = true;
+    }
+    const dim3 grid((unsigned)((long long)CL * p.query_tiles * p.c.tokens), p.c.kv_heads);
+    return launch(kern, grid, ATTEND_THREADS, L::BYTES, CL, stream, km, vm, p);
+}
+
+template <int DP, int NT, bool BF16>
+static cudaError_t launch_attend_cl(int cl, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t s) {
+    return cl == 8   ? launch_attend<DP, NT, BF16, 8>(km, vm, p, s)
+           : cl == 4 ? launch_attend<DP, NT, BF16, 4>(km, vm, p, s)
+           : cl == 2 ? launch_attend<DP, NT, BF16, 2>(km, vm, p, s)
+                     : launch_attend<DP, NT, BF16, 1>(km, vm, p, s);
+}
+
+static int pool_map(CUtensorMap* m, const FcsPagedCache* c, const void* base, const int64_t* stride) {
+    // (the stride of an axis of one entry says nothing; the contiguous one stands in for it)
+    int64_t st[3] = {stride[0], stride[1], stride[2]};
+    const int64_t size[3] = {c->pages, c->kv_heads, c->page_size};
+    int64_t dense = c->dim;
+    for (int i = 2; i >= 0; --i) {
+        if (size[i] == 1) st[i] = dense;
+        if (st[i] <= 0) return fail(FCS_ERR_INVALID_ARGUMENT, "strides of the pools must be positive");
+        dense = st[i] * size[i] > dense ? st[i] * size[i] : dense;
+    }
+    return make_tensor_map(m, base, c->dtype, c->pages, c->kv_heads, c->page_size, c->dim, st[0], st[1], st[2],
+                           c->page_size < TILE_KEYS ? c->page_size : TILE_KEYS);
+}
+
+static int attend(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const int* chosen, int k,
+                  float scale, void* out, const int64_t* out_stride, float* lse, int fill_tail, int* status, cudaStream_t stream) {
+    AttendParams p;
+    memset(&p, 0, sizeof(p));
+    int rc = check_cache(cache, p.c, status);
+    if (rc != FCS_OK) return rc;
+    if (!query_stride || !out_stride) return fail(FCS_ERR_INVALID_ARGUMENT, "query or out strides are NULL");
+    if ((rc = check_rows("query", query, query_stride, 2)) != FCS_OK) return rc;
+    if ((rc = check_rows("out", out, out_stride, 2)) != FCS_OK) return rc;
+    if ((rc = check_rows("key_pages", cache->key_pages, cache->key_stride, 3)) != FCS_OK) return rc;
+    if ((rc = check_rows("value_pages", cache->value_pages, cache->value_stride, 3)) != FCS_OK) return rc;
+    if ((rc = check_group(cache, q_heads)) != FCS_OK) return rc;
+    if (!chosen || k < 1) return fail(FCS_ERR_INVALID_ARGUMENT, "chosen is NULL or has no entries (k=%d)", k);
+    if (scale != scale) return fail(FCS_ERR_INVALID_ARGUMENT, "scale is not a number");
+    p.query = static_cast<const uint16_t*>(query);
+    p.out = static_cast<uint16_t*>(out);
+    for (int i = 0; i < 2; ++i) {
+        p.query_st[i] = query_stride[i];
+        p.out_st[i] = out_stride[i];
+    }
+    p.lse = lse;
+    p.chosen = chosen;
+    p.k = k;
+    p.group = q_heads / cache->kv_heads;
+    p.q_heads = q_heads;
+    p.c_log2 = scale * 1.4426950408889634f;
+    p.fill_tail = fill_tail;
+    const int nt = p.group > 8 ? 2 : 1;
+    p.query_tiles = (p.group + 8 * nt - 1) / (8 * nt);
+    // CTAs of a row: as many as the device has room for, two tiles of keys for each at least
+    const long long rows = (long long)cache->tokens * cache->kv_heads * p.query_tiles;
+    const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
+    int cl = 1;
+    while (cl < 8 && rows * cl * 2 <= 2ll * num_sms() && tiles >= 4ll * cl) cl *= 2;
+    if (rows / cache->kv_heads * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
+    CUtensorMap km, vm;
+    if ((rc = pool_map(&km, cache, cache->key_pages, cache->key_stride)) != FCS_OK) return rc;
+    if ((rc = pool_map(&vm, cache, cache->value_pages, cache->value_stride)) != FCS_OK) return rc;
+    const bool wide = cache->dim > 64, bf16 = cache->dtype == FCS_DTYPE_BF16;
+    cudaError_t e;
+    if (wide)
+        e = nt == 1 ? (bf16 ? launch_attend_cl<128, 1, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 1, false>(cl, km, vm, p, stream))
+                    : (bf16 ? launch_attend_cl<128, 2, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 2, false>(cl, km, vm, p, stream));
+    else
+        e = nt == 1 ? (bf16 ? launch_attend_cl<64, 1, true>(cl, km, vm, p, stream) : launch_attend_cl<64, 1, false>(cl, km, vm, p, stream))
+                    : (bf16 ? launch_attend_cl<64, 2, true>(cl, km, vm, p, stream) : launch_attend_cl<64, 2, false>(cl, km, vm, p, stream));
+    if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "attending failed to launch: %s", cudaGetErrorString(e));
+    return FCS_OK;
+}
+
+}  // namespace paged
+}  // namespace fcs
+
+extern "C" {
+
+int fcs_append_paged(const FcsPagedCache* cache, const FcsPagedRows* rows, int* status, void* stream) {
+    fcs::g_err[0] = 0;
+    return fcs::paged::append(cache, rows, status, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t fcs_select_pages_workspace_bytes(const FcsPagedCache* cache) {
+    if (!cache || cache->tokens <= 0 || cache->kv_heads <= 0 || cache->table_width <= 0) return 0;
+    return fcs::paged::select_workspace(cache);
+}
+
+int fcs_select_pages(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const void* bounds,
+                     int k, int first, int last, int* chosen, int fill_tail, void* workspace, size_t workspace_bytes, int* status,
+                     void* stream) {
+    fcs::g_err[0] = 0;
+    return fcs::paged::select(cache, query, query_stride, q_heads, bounds, k, first, last, chosen, fill_tail, workspace,
+                              workspace_bytes, status, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int fcs_attend_pages(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const int* chosen, int k,
+                     float scale, void* out, const int64_t* out_stride, float* lse, int fill_tail, int* status, void* stream) {
+    fcs::g_err[0] = 0;
+    return fcs::paged::attend(cache, query, query_stride, q_heads, chosen, k, scale, out, out_stride, lse, fill_tail, status,
+                              reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -30,6 +30,10 @@ FcsRunHostCallFn g_run_host_call = nullptr;
 FcsSelectTopkFn g_select_topk = nullptr;
 FcsSelectThresholdFn g_select_threshold = nullptr;
 FcsLastErrorFn g_last_error = nullptr;
+FcsAppendPagedFn g_append_paged = nullptr;
+FcsSelectPagesWorkspaceFn g_select_pages_workspace = nullptr;
+FcsSelectPagesFn g_select_pages = nullptr;
+FcsAttendPagesFn g_attend_pages = nullptr;
 
 constexpr int MAX_DEVICES = 64;
 int* g_status[MAX_DEVICES] = {nullptr};   // the device status words (owned by the Python package)
@@ -49,6 +53,10 @@ PyObject* raise_library_error(int rc) {
 at::Tensor empty_f32(int64_t rows, int64_t cols, c10::Device dev) {
     const int64_t size[2] = {rows, cols};
     return at::detail::empty_cuda(c10::IntArrayRef(size, 2), at::kFloat, dev, std::nullopt);
+}
+
+at::Tensor empty_on(c10::IntArrayRef size, at::ScalarType type, c10::Device dev) {
+    return at::detail::empty_cuda(size, type, dev, std::nullopt);
 }
 
 // Scratch of one call; freed when the call returns (the caching allocator hands it out again in
@@ -342,6 +350,280 @@ PyObject* py_threshold(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the paged cache
+
+// A tensor argument that may be None; `ok` falls where it is neither.
+const at::Tensor* optional_tensor(PyObject* o, bool& ok) {
+    if (o == Py_None) return nullptr;
+    if (!usable(o)) {
+        ok = false;
+        return nullptr;
+    }
+    return &THPVariable_Unpack(o);
+}
+
+bool indices_ok(const at::Tensor& t, int64_t dims, c10::Device dev) {
+    return t.dim() == dims && t.scalar_type() == at::kInt && t.device() == dev && t.numel() > 0;
+}
+
+// Rows of 16-bit elements that are read in pieces of 16 bytes: unit inner stride, the other strides multiples of 8.
+template <int N>
+bool rows_ready(const at::Tensor& t, int64_t (&st)[N]) {
+    int64_t any = 0;
+    for (int i = 0; i < N; ++i) {
+        st[i] = t.size(i) > 1 ? t.stride(i) : 0;      // (the stride of an axis of one entry says nothing)
+        if (st[i] < 0) return false;
+        any |= st[i];
+    }
+    return (t.size(N) == 1 || t.stride(N) == 1) && any % 8 == 0 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0;
+}
+
+// A pool as the kernels take it: positive strides, no two entries in one place as far as the strides say.
+bool pool_ready(const at::Tensor& t, int64_t (&st)[3]) {
+    if (!rows_ready<3>(t, st)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (t.size(i) > 1 && st[i] < t.size(3)) return false;
+    return true;
+}
+
+// The batch and, unless they are not given, the pools of a call; whatever had to be laid out anew is held until it returns.
+struct PagedArgs {
+    FcsPagedCache c = {};
+    at::Tensor table, lens, starts;
+    c10::Device dev = c10::Device(c10::kCPU);
+    int* status = nullptr;
+
+    bool batch(const at::Tensor& rows, const at::Tensor& t, const at::Tensor& n, const at::Tensor* s) {
+        dev = rows.device();
+        const int idx = dev.index();
+        if (!dev.is_cuda() || idx < 0 || idx >= MAX_DEVICES || !g_status[idx] || !g_append_paged) return false;
+        if (rows.dim() != 3 || !indices_ok(t, 2, dev) || !indices_ok(n, 1, dev)) return false;
+        const int64_t T = rows.size(0), B = n.size(0), D = rows.size(2);
+        if (T < 1 || T > 0x7fffffffLL || B > 0x7fffffffLL || t.size(0) != B || t.size(1) > 0x7fffffffLL) return false;
+        if (D % 8 || D < 8 || D > 128 || (rows.scalar_type() != at::kHalf && rows.scalar_type() != at::kBFloat16)) return false;
+        if (s ? !indices_ok(*s, 1, dev) || s->size(0) != B + 1 : T != B) return false;
+        status = g_status[idx];
+        table = t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
+        if (B > 1 && table.stride(0) < t.size(1)) table = t.contiguous();
+        lens = n.contiguous();
+        if (s) starts = s->contiguous();
+        c.page_table = static_cast<const int*>(table.const_data_ptr());
+        c.table_stride = B > 1 ? table.stride(0) : t.size(1);
+        c.lens = static_cast<const int*>(lens.const_data_ptr());
+        c.starts = s ? static_cast<const int*>(starts.const_data_ptr()) : nullptr;
+        c.dim = (int)D;
+        c.dtype = dtype_code(rows.scalar_type());
+        c.sequences = (int)B;
+        c.table_width = (int)t.size(1);
+        c.tokens = (int)T;
+        return true;
+    }
+    bool pools(const at::Tensor& rows, const at::Tensor& k, const at::Tensor& v) {
+        if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.device() != dev || v.device() != dev) return false;
+        if (k.scalar_type() != rows.scalar_type() || v.scalar_type() != rows.scalar_type()) return false;
+        const auto n = k.sizes();
+        if (n[0] < 1 || n[0] > 0x7fffffffLL || n[1] < 1 || n[1] > 65535 || n[3] != c.dim) return false;
+        if (n[2] != 16 && n[2] != 32 && n[2] != 64 && n[2] != 128) return false;
+        if (!pool_ready(k, c.key_stride) || !pool_ready(v, c.value_stride)) return false;
+        c.key_pages = const_cast<void*>(k.const_data_ptr());
+        c.value_pages = const_cast<void*>(v.const_data_ptr());
+        c.pages = (int)n[0];
+        c.kv_heads = (int)n[1];
+        c.page_size = (int)n[2];
+        return true;
+    }
+    bool heads_ok(const at::Tensor& query) const {
+        return query.size(1) > 0 && query.size(1) % c.kv_heads == 0 && query.size(1) <= 0x7ffffLL;
+    }
+    void* stream() const { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+};
+
+bool like_rows(const at::Tensor& t, const at::Tensor& rows) {
+    return t.dim() == 3 && t.size(0) == rows.size(0) && t.size(2) == rows.size(2) && t.device() == rows.device() &&
+           t.scalar_type() == rows.scalar_type();
+}
+
+int int_or(PyObject* o, bool& ok) {
+    const long long v = PyLong_CheckExact(o) ? PyLong_AsLongLong(o) : -1;
+    if (v < 0 || v > 0x7fffffffLL) {
+        PyErr_Clear();
+        ok = false;
+    }
+    return (int)v;
+}
+
+// append_paged(key, value, key_pages, value_pages, page_table, lens, starts, query, cos, sin, positions, interleaved,
+// bounds, query_out) -> rotated query, or True without one
+PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 14) Py_RETURN_NONE;
+    for (int i = 0; i < 6; ++i)
+        if (!usable(args[i])) Py_RETURN_NONE;
+    bool ok = true;
+    const at::Tensor *starts = optional_tensor(args[6], ok), *query_in = optional_tensor(args[7], ok),
+                     *cos = optional_tensor(args[8], ok), *sin = optional_tensor(args[9], ok),
+                     *positions = optional_tensor(args[10], ok), *bounds = optional_tensor(args[12], ok),
+                     *query_out = optional_tensor(args[13], ok);
+    const int interleaved = PyObject_IsTrue(args[11]);
+    if (interleaved < 0) return nullptr;
+    if (!ok) Py_RETURN_NONE;
+    at::Tensor key = THPVariable_Unpack(args[0]), value = THPVariable_Unpack(args[1]), query, out, where;
+    PagedArgs a;
+    FcsPagedRows r = {};
+    int rc;
+    {
+        const c10::OptionalDeviceGuard guard(key.is_cuda() ? std::optional<c10::Device>(key.device()) : std::nullopt);
+        if (!a.batch(key, THPVariable_Unpack(args[4]), THPVariable_Unpack(args[5]), starts)) Py_RETURN_NONE;
+        if (!a.pools(key, THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]))) Py_RETURN_NONE;
+        if (!like_rows(value, key) || key.size(1) != a.c.kv_heads || value.size(1) != a.c.kv_heads) Py_RETURN_NONE;
+        if ((cos == nullptr) != (sin == nullptr) || (positions && !cos)) Py_RETURN_NONE;
+        if (cos) {
+            if (cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->scalar_type() != at::kFloat ||
+                sin->scalar_type() != at::kFloat || cos->device() != a.dev || sin->device() != a.dev || !cos->is_contiguous() ||
+                !sin->is_contiguous() || cos->size(0) < 1 || cos->size(0) > 0x7fffffffLL || cos->size(1) < 8 ||
+                cos->size(1) % 8 || 2 * cos->size(1) > a.c.dim ||
+                ((reinterpret_cast<uintptr_t>(cos->const_data_ptr()) | reinterpret_cast<uintptr_t>(sin->const_data_ptr())) & 15))
+                Py_RETURN_NONE;
+            r.cos = static_cast<const float*>(cos->const_data_ptr());
+            r.sin = static_cast<const float*>(sin->const_data_ptr());
+            r.table_rows = (int)cos->size(0);
+            r.rotary = 2 * (int)cos->size(1);
+            r.interleaved = interleaved;
+            if (positions) {
+                if (!indices_ok(*positions, 1, a.dev) || positions->size(0) != key.size(0)) Py_RETURN_NONE;
+                where = positions->contiguous();
+                r.positions = static_cast<const int*>(where.const_data_ptr());
+            }
+        }
+        if (bounds) {
+            if (bounds->dim() != 4 || bounds->size(0) != a.c.pages || bounds->size(1) != a.c.kv_heads || bounds->size(2) != 2 ||
+                bounds->size(3) != a.c.dim || bounds->scalar_type() != key.scalar_type() || bounds->device() != a.dev ||
+                !bounds->is_contiguous() || (reinterpret_cast<uintptr_t>(bounds->const_data_ptr()) & 15))
+                Py_RETURN_NONE;
+            r.bounds = const_cast<void*>(bounds->const_data_ptr());
+        }
+        if (query_out && !query_in) Py_RETURN_NONE;
+        if (query_in) {
+            if (!like_rows(*query_in, key) || !a.heads_ok(*query_in)) Py_RETURN_NONE;
+            if (query_out && (!like_rows(*query_out, key) || query_out->size(1) != query_in->size(1) ||
+                              !rows_ready<2>(*query_out, r.query_out_stride)))
+                Py_RETURN_NONE;
+            query = rows_ready<2>(*query_in, r.query_stride) ? *query_in : query_in->contiguous();
+            rows_ready<2>(query, r.query_stride);
+            r.fill_tail = query_out == nullptr;
+            out = query_out ? *query_out : empty_on(query.sizes(), query.scalar_type(), a.dev);
+            rows_ready<2>(out, r.query_out_stride);
+            r.query = query.const_data_ptr();
+            r.query_out = out.mutable_data_ptr();
+            r.q_heads = (int)query.size(1);
+        }
+        if (!rows_ready<2>(key, r.key_stride)) key = key.contiguous();
+        if (!rows_ready<2>(value, r.value_stride)) value = value.contiguous();
+        rows_ready<2>(key, r.key_stride);
+        rows_ready<2>(value, r.value_stride);
+        r.key = key.const_data_ptr();
+        r.value = value.const_data_ptr();
+        WithoutGil nogil;
+        rc = g_append_paged(&a.c, &r, a.status, a.stream());
+    }
+    if (rc != FCS_OK) return raise_library_error(rc);
+    if (!query_in) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// select_pages(query, bounds, page_table, lens, k, page_size, starts, first, last, out) -> (tokens, kv_heads, k)
+PyObject* py_select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) Py_RETURN_NONE;
+    for (int i = 0; i < 4; ++i)
+        if (!usable(args[i])) Py_RETURN_NONE;
+    bool ok = true;
+    const int k = int_or(args[4], ok), page_size = int_or(args[5], ok), first = int_or(args[7], ok), last = int_or(args[8], ok);
+    const at::Tensor *starts = optional_tensor(args[6], ok), *given = optional_tensor(args[9], ok);
+    if (!ok || k < 1 || last < 1 || (int64_t)first + last > k) Py_RETURN_NONE;
+    at::Tensor query = THPVariable_Unpack(args[0]), out;
+    const at::Tensor& bounds = THPVariable_Unpack(args[1]);
+    PagedArgs a;
+    int rc;
+    {
+        const c10::OptionalDeviceGuard guard(query.is_cuda() ? std::optional<c10::Device>(query.device()) : std::nullopt);
+        if (!a.batch(query, THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]), starts)) Py_RETURN_NONE;
+        if (bounds.dim() != 4 || bounds.size(0) < 1 || bounds.size(0) > 0x7fffffffLL || bounds.size(1) < 1 ||
+            bounds.size(1) > 65535 || bounds.size(2) != 2 || bounds.size(3) != a.c.dim ||
+            bounds.scalar_type() != query.scalar_type() || bounds.device() != a.dev || !bounds.is_contiguous() ||
+            (reinterpret_cast<uintptr_t>(bounds.const_data_ptr()) & 15))
+            Py_RETURN_NONE;
+        if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) Py_RETURN_NONE;
+        a.c.pages = (int)bounds.size(0);
+        a.c.kv_heads = (int)bounds.size(1);
+        a.c.page_size = page_size;
+        if (!a.heads_ok(query)) Py_RETURN_NONE;
+        const int64_t size[3] = {query.size(0), bounds.size(1), k};
+        if (given && (given->sizes() != c10::IntArrayRef(size, 3) || given->scalar_type() != at::kInt || given->device() != a.dev ||
+                      !given->is_contiguous()))
+            Py_RETURN_NONE;
+        out = given ? *given : empty_on(c10::IntArrayRef(size, 3), at::kInt, a.dev);
+        int64_t st[2];
+        if (!rows_ready<2>(query, st)) query = query.contiguous();
+        rows_ready<2>(query, st);
+        const int64_t bytes[1] = {(int64_t)g_select_pages_workspace(&a.c)};
+        const at::Tensor scratch = empty_on(c10::IntArrayRef(bytes, 1), at::kByte, a.dev);
+        WithoutGil nogil;
+        rc = g_select_pages(&a.c, query.const_data_ptr(), st, (int)query.size(1), bounds.const_data_ptr(), k, first, last,
+                            static_cast<int*>(out.mutable_data_ptr()), given == nullptr, scratch.mutable_data_ptr(),
+                            (size_t)bytes[0], a.status, a.stream());
+    }
+    if (rc != FCS_OK) return raise_library_error(rc);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// attend_pages(query, key_pages, value_pages, page_table, lens, pages, starts, scale, with_lse, out) -> out, or (out, lse)
+PyObject* py_attend_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10) Py_RETURN_NONE;
+    for (int i = 0; i < 6; ++i)
+        if (!usable(args[i])) Py_RETURN_NONE;
+    bool ok = true;
+    const at::Tensor *starts = optional_tensor(args[6], ok), *given = optional_tensor(args[9], ok);
+    const int with_lse = PyObject_IsTrue(args[8]);
+    if (with_lse < 0) return nullptr;
+    if (!ok) Py_RETURN_NONE;
+    at::Tensor query = THPVariable_Unpack(args[0]), out, lse, pages;
+    if (query.dim() != 3) Py_RETURN_NONE;
+    const double scale = args[7] == Py_None ? 1.0 / std::sqrt((double)query.size(2)) : PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (std::isnan(scale)) Py_RETURN_NONE;
+    const at::Tensor& chosen = THPVariable_Unpack(args[5]);
+    PagedArgs a;
+    int rc;
+    {
+        const c10::OptionalDeviceGuard guard(query.is_cuda() ? std::optional<c10::Device>(query.device()) : std::nullopt);
+        if (!a.batch(query, THPVariable_Unpack(args[3]), THPVariable_Unpack(args[4]), starts)) Py_RETURN_NONE;
+        if (!a.pools(query, THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2])) || !a.heads_ok(query)) Py_RETURN_NONE;
+        if (!indices_ok(chosen, 3, a.dev) || chosen.size(0) != query.size(0) || chosen.size(1) != a.c.kv_heads ||
+            chosen.size(2) > 0x7fffffffLL / 256)
+            Py_RETURN_NONE;
+        int64_t st[2], out_st[2];
+        if (given && (!like_rows(*given, query) || given->size(1) != query.size(1) || !rows_ready<2>(*given, out_st))) Py_RETURN_NONE;
+        if (!rows_ready<2>(query, st)) query = query.contiguous();
+        rows_ready<2>(query, st);
+        pages = chosen.contiguous();
+        out = given ? *given : empty_on(query.sizes(), query.scalar_type(), a.dev);
+        rows_ready<2>(out, out_st);
+        if (with_lse) lse = empty_f32(query.size(0), query.size(1), a.dev);
+        WithoutGil nogil;
+        rc = g_attend_pages(&a.c, query.const_data_ptr(), st, (int)query.size(1), static_cast<const int*>(pages.const_data_ptr()),
+                            (int)pages.size(2), (float)scale, out.mutable_data_ptr(), out_st,
+                            with_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr, given ? 2 : 3, a.status, a.stream());
+    }
+    if (rc != FCS_OK) return raise_library_error(rc);
+    if (!with_lse) return THPVariable_Wrap(std::move(out));
+    return pair(std::move(out), std::move(lse));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(handle): the entry points of the loaded CUDA library (a dlopen handle)
 PyObject* py_bind(PyObject*, PyObject* arg) {
     void* h = PyLong_AsVoidPtr(arg);
@@ -352,7 +634,12 @@ PyObject* py_bind(PyObject*, PyObject* arg) {
     g_select_threshold = reinterpret_cast<FcsSelectThresholdFn>(sym("fcs_select_threshold"));
     g_run_call = reinterpret_cast<FcsRunCallFn>(sym("fcs_run_call"));
     g_run_host_call = reinterpret_cast<FcsRunHostCallFn>(sym("fcs_run_host_call"));
-    if (!g_last_error || !g_select_topk || !g_select_threshold || !g_run_call || !g_run_host_call) {
+    g_append_paged = reinterpret_cast<FcsAppendPagedFn>(sym("fcs_append_paged"));
+    g_select_pages_workspace = reinterpret_cast<FcsSelectPagesWorkspaceFn>(sym("fcs_select_pages_workspace_bytes"));
+    g_select_pages = reinterpret_cast<FcsSelectPagesFn>(sym("fcs_select_pages"));
+    g_attend_pages = reinterpret_cast<FcsAttendPagesFn>(sym("fcs_attend_pages"));
+    if (!g_last_error || !g_select_topk || !g_select_threshold || !g_run_call || !g_run_host_call || !g_append_paged ||
+        !g_select_pages_workspace || !g_select_pages || !g_attend_pages) {
         PyErr_SetString(PyExc_RuntimeError, "flash_colsum_b200: the CUDA library lacks an entry point of this binding");
         return nullptr;
     }
@@ -378,6 +665,9 @@ PyMethodDef g_methods[] = {
     {"host", fast(py_host), METH_FASTCALL, nullptr},
     {"topk", fast(py_topk), METH_FASTCALL, nullptr},
     {"threshold", fast(py_threshold), METH_FASTCALL, nullptr},
+    {"append_paged", fast(py_append_paged), METH_FASTCALL, nullptr},
+    {"select_pages", fast(py_select_pages), METH_FASTCALL, nullptr},
+    {"attend_pages", fast(py_attend_pages), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_O, nullptr},
     {"set_status", fast(py_set_status), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

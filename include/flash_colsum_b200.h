@@ -60,6 +60,10 @@ extern "C" {
 #define FCS_STATUS_WAIT_MMA 2
 #define FCS_STATUS_WAIT_CONSUMER 3
 #define FCS_STATUS_WAIT_PEER 4
+/* ... or by a kernel over a paged cache: a page that a token needs is not in the table or lies
+ * outside the pools; a position that the rotation's tables do not have. */
+#define FCS_STATUS_BAD_PAGE 5
+#define FCS_STATUS_BAD_POSITION 6
 
 /* Library version, as major * 10000 + minor * 100 + patch. */
 int fcs_version(void);
@@ -322,6 +326,92 @@ int fcs_select_topk(const float *colsum, int64_t ld, int B, int S, int k,
  */
 int fcs_select_threshold(const float *colsum, int64_t ld, int B, int S, float threshold, int relative,
                          int *indices, int *counts, void *stream);
+
+/*
+ * A cache of keys and values in pages, and the attention that reads a part of it: a step's keys
+ * and values are appended (fcs_append_paged), every query chooses the pages that promise it the
+ * largest scores (fcs_select_pages), and attends over those alone (fcs_attend_pages).  What token
+ * pruning by column means does once for a prompt, this does for every query.  No counterpart in the
+ * reference.
+ *
+ * The batch: `sequences` sequences whose new tokens lie one behind the other in the rows of key,
+ * value and query -- sequence b owns rows starts[b] .. starts[b+1] - 1, or row b alone when starts is
+ * NULL (tokens == sequences then).  lens[b] counts the tokens of sequence b in the cache, the new
+ * ones included, so that row t of sequence b has position lens[b] - starts[b+1] + t (lens[b] - 1
+ * without starts).  Rows from starts[sequences] on belong to nobody: inputs are not read there, and
+ * outputs are left as they are, or set (rotated queries and results 0, pages -1) when fill_tail is 1.
+ * Position i of sequence b lies in page page_table[b * table_stride + i / page_size], slot
+ * i % page_size.  starts ascends, starts[0] is 0; page_table, lens and starts are device memory.
+ *
+ * The pools are (pages, kv_heads, page_size, dim) tensors of 16-bit elements with unit inner stride;
+ * the strides of page, head and slot are multiples of 8, in any order.  page_size is 16, 32, 64 or
+ * 128, dim a multiple of 8 up to 128.  The heads of a query share the keys of head / group, group =
+ * q_heads / kv_heads.
+ *
+ * A page that a token needs and the table does not have (an entry outside 0 .. pages - 1, or a
+ * position past the table's width) sets *status to FCS_STATUS_BAD_PAGE; nothing is written to it, and
+ * nothing read from it enters a result.
+ */
+typedef struct FcsPagedCache {
+    void *key_pages, *value_pages;
+    int64_t key_stride[3], value_stride[3];
+    const int *page_table;
+    int64_t table_stride;
+    const int *lens;
+    const int *starts;
+    int pages, kv_heads, page_size, dim, dtype;
+    int sequences, table_width, tokens;
+} FcsPagedCache;
+
+/*
+ * key, value: (tokens, kv_heads, dim); query, query_out: (tokens, q_heads, dim), or NULL both.
+ * cos, sin: fp32 (table_rows, rotary / 2), contiguous, or NULL for no rotation.  The first `rotary`
+ * features (a multiple of 16) of keys and queries are rotated by row positions[t] of the tables, or
+ * by the row of the token's position when positions is NULL: feature i with feature i + rotary / 2,
+ * or 2 i with 2 i + 1 when `interleaved`.  A token whose row the tables do not have is not appended,
+ * its query comes out as zeros, and *status is FCS_STATUS_BAD_POSITION.  query_out may be query.
+ * bounds: (pages, kv_heads, 2, dim), contiguous, of the cache's type, or NULL: per feature the
+ * smallest and the largest of the keys written to a page since its slot 0 was.
+ */
+typedef struct FcsPagedRows {
+    const void *key, *value, *query;
+    void *query_out;
+    int64_t key_stride[2], value_stride[2], query_stride[2], query_out_stride[2];
+    int q_heads;
+    const float *cos, *sin;
+    int table_rows, rotary, interleaved;
+    const int *positions;
+    void *bounds;
+    int fill_tail;
+} FcsPagedRows;
+
+int fcs_append_paged(const FcsPagedCache *cache, const FcsPagedRows *rows, int *status, void *stream);
+
+/*
+ * Per token and key/value head the k pages to attend to, as indices into the sequence's row of the
+ * table: chosen[tokens][kv_heads][k], ascending, -1 behind the last.  Of the pages up to the token's
+ * own the `first` first and the `last` last are always chosen (last counts the token's own page, and is 1
+ * at least), the rest by the largest sum over the group's queries of sum_d max(q_d low_d, q_d high_d),
+ * which no sum of scores with keys of the page exceeds.  Ties go to the lower page, a score that is NaN counts as
+ * +inf, one of a page that the table lacks as -inf.  Scores are summed in 64 bits.  Of `cache` the pools are not
+ * read.  workspace: fcs_select_pages_workspace_bytes(cache) bytes, 16-byte aligned.
+ */
+size_t fcs_select_pages_workspace_bytes(const FcsPagedCache *cache);
+int fcs_select_pages(const FcsPagedCache *cache, const void *query, const int64_t *query_stride, int q_heads,
+                     const void *bounds, int k, int first, int last, int *chosen, int fill_tail,
+                     void *workspace, size_t workspace_bytes, int *status, void *stream);
+
+/*
+ * Softmax attention of every query over the keys of its chosen pages that are not behind its own
+ * position: out (tokens, q_heads, dim) of the cache's type; lse fp32 (tokens, q_heads), the natural
+ * logarithm of the sum of exp(scale * score), or NULL.  chosen[tokens][kv_heads][k] in any order;
+ * entries below 0 and pages behind the token's own weigh nothing, a page that is listed twice weighs
+ * twice.  A query without a key gets zeros and an lse of -inf.  fill_tail is a sum: 1 for the rows of out behind the
+ * last sequence, 2 for those of lse (-inf).
+ */
+int fcs_attend_pages(const FcsPagedCache *cache, const void *query, const int64_t *query_stride, int q_heads,
+                     const int *chosen, int k, float scale, void *out, const int64_t *out_stride, float *lse,
+                     int fill_tail, int *status, void *stream);
 
 /*
  * Measurement aids.  No counterpart in the reference, which times whole calls
