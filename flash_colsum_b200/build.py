@@ -33,7 +33,7 @@ UNITS = {
         "sm100_ptx.cuh", "schedule.h", "colsum_small_q.cuh", "colsum_few_rows.cuh", "round_fp32.cuh", "colsum_math.cuh",
         "colsum_single_pass.cuh", "select_topk.cuh", "colsum_fused_short.cuh", "host_api.h", "host_common.h") + [_ABI],
     _csrc("paged_sm100.cu")[0]: _csrc(
-        "sm100_ptx.cuh", "paged.cuh", "paged_append.cuh", "paged_select.cuh", "paged_attend.cuh",
+        "sm100_ptx.cuh", "paged.cuh", "paged_mma.cuh", "paged_append.cuh", "paged_select.cuh", "paged_attend.cuh",
         "host_common.h") + [_ABI],
 }
 SOURCES = list(UNITS)

@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace fcs {
 namespace paged {
@@ -51,47 +52,6 @@ struct AttendLayout {
     static constexpr int BYTES = OFF_FLAG + 16 + 1024;              // (1024: alignment of the swizzled tiles)
 };
 
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-    uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-    return r;
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// Two values as 16-bit ones, and what their rounding leaves.
-template <bool BF16>
-__device__ __forceinline__ uint32_t round_pair(float a, float b, float& ra, float& rb) {
-    if constexpr (BF16) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
-        ra = a - __uint_as_float(w << 16);
-        rb = b - __uint_as_float(w & 0xffff0000u);
-        return w;
-    } else {
-        const __half2 v = __floats2half2_rn(a, b);
-        const float2 f = __half22float2(v);
-        ra = a - f.x;
-        rb = b - f.y;
-        return *reinterpret_cast<const uint32_t*>(&v);
-    }
-}
 template <bool BF16>
 __device__ __forceinline__ uint16_t round_one(float a) {
     if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(a));

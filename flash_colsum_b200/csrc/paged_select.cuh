@@ -1,15 +1,27 @@
 // Choosing pages: per query and key/value head the k pages whose bounds promise the largest scores.
 //
 // The mathematics: over the keys of a page q . k <= sum_d max(q_d low_d, q_d high_d); summed over the queries of a group
-// that is p . high - n . low with p = sum max(q, 0) and n = sum max(-q, 0), one product of 2 D terms for the whole
-// group.  The first and the last pages of a query are always chosen; of the others the best, the lower page among
-// equals.  Which of two pages is the better one must not hang on the order of a sum, so the scores are summed in 64 bits.
+// that is n . low + p . high with n = sum min(q, 0) and p = sum max(q, 0), one product of 2 D terms for the whole group.
+// The first and the last pages of a query are always chosen; of the others the best, the lower page among equals.
+//
+// Which of two pages is the better one must not hang on the order of a sum: pages are ordered by scores summed in 64 bits.  Few
+// need that.  Scores are summed in 32 bits first, which are off by at most
+//     E = c (sum |n| + sum |p|) max |bound|,
+// c counting the roundings; with t the k-th largest of them, a page above t + 2 E is chosen and one below t - 2 E is not whatever
+// the exact scores are (the k-th largest of numbers each moved by E moves by E at most), and only the pages between are summed
+// again, in 64 bits.  Where E is not finite, all are.
+//
+// Two forms share that.  Few tokens a sequence (select_row_kernel): a cluster per row reads the bounds once, a warp
+// a page, and the first CTA chooses.  Many (score_tiles_kernel, choose_kernel): 64 tokens by 64 pages at a time on
+// tensor cores, n and p in two 16-bit parts each, and a warp or a block per row chooses from the scores.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <float.h>
 
 #include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace fcs {
 namespace paged {
@@ -22,191 +34,782 @@ struct SelectParams {
     int group;                      // query heads of a key/value head
     int k, first, last;
     int* chosen;                    // (tokens, kv_heads, k)
-    double* scores;                 // (tokens of this launch, kv_heads, width)
-    int t0;                         // first token of this launch
+    double* exact;                  // (tokens of this launch, kv_heads, pitch): sums in 64 bits, where they are needed
+    float* scores;                  // the same of sums in 32 bits (not for select_row_kernel)
+    float* errors;                  // (tokens of this launch, kv_heads, splits): E
+    int pitch, splits;
+    int t0, t1;                     // tokens of this launch
     int fill_tail;
 };
-
-constexpr int SCORE_THREADS = 256;
-constexpr int SCORE_PAGES = 64;     // pages of a CTA: eight of a warp
 
 template <bool BF16>
 __device__ __forceinline__ float widen16(uint32_t v) {     // (the low half of v)
     if constexpr (BF16) return __uint_as_float(v << 16);
     return __half2float(__ushort_as_half((unsigned short)v));
 }
-
+template <bool BF16>
+__device__ __forceinline__ float2 widen_pair(uint32_t v) {
+    if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
 // Pages that the query at `pos` sees (all of them, whether the table holds them or not).
 __device__ __forceinline__ long long pages_seen(const Batch& c, long long pos) {
     return pos < 0 ? 0 : (pos >> c.page_shift) + 1;
 }
 
-// grid: (page chunks, kv heads, tokens)
-template <bool BF16>
-__global__ void __launch_bounds__(SCORE_THREADS) score_kernel(const __grid_constant__ SelectParams p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const Batch& c = p.c;
-    const int D = c.dim, h = blockIdx.y, t = p.t0 + (int)blockIdx.z;
-    const int b = sequence_of(c, t);
-    if (b >= c.sequences) return;
-    const long long seen = min(pages_seen(c, position_of(c, b, t)), (long long)c.width);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int base = (int)blockIdx.x * SCORE_PAGES + warp * (SCORE_PAGES / 8);
-    if (base >= seen) return;
+// Pages of a row: 0 .. pages - 1 are there, lo .. hi - 1 of them compete for `need` places, the rest is chosen.
+struct Row {
+    int t, h, b;
+    int pages, lo, hi;
+    uint32_t need;
+    __device__ void set(const SelectParams& p, int t_, int h_, int b_, long long pos) {
+        t = t_, h = h_, b = b_;
+        const long long seen = pages_seen(p.c, pos);
+        pages = (int)min(seen, (long long)p.c.width);
+        lo = min(p.first, pages);
+        hi = (int)max((long long)lo, min((long long)pages, seen - p.last));
+        need = (uint32_t)max(0, p.k - lo - (pages - hi));
+    }
+};
 
-    // A lane keeps eight of the 2 D features -- the first D meet the lows, the others the highs; 2 D / 8 lanes or
-    // the next power of two hold a page, and a warp as many pages at a time as fit.
-    const int vectors = D / 4;
-    int span = 2;
-    while (span < vectors) span *= 2;
-    const int v = lane & (span - 1);
-    double part[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part[i] = 0.0;
-    if (v < vectors) {
-        const bool low = v < vectors / 2;
-        const uint16_t* q = p.query + t * p.query_st[0] + (long long)h * p.group * p.query_st[1] + (low ? v : v - vectors / 2) * 8;
+// Order-preserving keys: larger value, larger key; NaN is +inf, zeros are equal.  No value has key 0.
+__device__ __forceinline__ uint32_t key_of(float s) {
+    const uint32_t bits = __float_as_uint(s != s ? INFINITY : s == 0.f ? 0.f : s);
+    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ unsigned long long key_of(double s) {
+    const unsigned long long bits = (unsigned long long)__double_as_longlong(s != s ? (double)INFINITY : s == 0.0 ? 0.0 : s);
+    return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
+}
+
+// E for a row whose parts sum up to `size` in magnitude, over pages whose bounds reach up to `reach`.  Sums that may overflow
+// are no sums (NaN likewise), and products that underflow lose what no share of the whole covers: 1e-36 is 85 times
+// the smallest normal number.
+__device__ __forceinline__ float error_of(float c, float size, float reach) {
+    const float most = size * reach;
+    return most < 1e37f ? c * most + 1e-36f : INFINITY;
+}
+
+// E of scores that matrix instructions formed of parts in two 16-bit pieces, 16 terms at a time.  Roundings of 2^-24: the group's
+// sums and the additions of D / 8 steps; in a step up to 2^-23 of each of 17 terms, where a tensor core drops what lies below the
+// last bit of the largest; what the pieces leave, 2^-18 (bf16) or 2^-22 (fp16) of a part, and half of fp16's smallest step of
+// every part.
+template <bool BF16>
+__device__ __forceinline__ float score_error(const SelectParams& p, float size, float reach) {
+    const float error = error_of((float)(p.group + p.c.dim / 8 + 36) * 6.5e-8f + (BF16 ? 3.9e-6f : 2.4e-7f), size, reach);
+    if constexpr (BF16) return error;
+    return size < 6e4f ? error + 2.f * p.c.dim * 3e-8f * reach : INFINITY;
+}
+
+// The largest magnitude among 16-bit values whose bit patterns, as unsigned and as signed integers, go up to these pairs: the
+// one finds the largest negative, the other the largest positive value.  NaN comes out as such or as an infinity.
+template <bool BF16>
+__device__ __forceinline__ float reach_of(uint32_t as_unsigned, uint32_t as_signed) {
+    const uint32_t a = as_unsigned & 0x7fff7fffu, b = as_signed & 0x7fff7fffu;
+    // (no negative value: the unsigned maximum is the largest positive one, and the other way round)
+    const float2 x = widen_pair<BF16>(a), y = widen_pair<BF16>(b);
+    return max_or_nan(max_or_nan(x.x, x.y), max_or_nan(y.x, y.y));
+}
+
+// A page's score in 64 bits, by a warp.
+template <bool BF16>
+__device__ double exact_score(const SelectParams& p, const Row& r, int i) {
+    const Batch& c = p.c;
+    const int page = physical_page(c, r.b, i);
+    if (page < 0) return -INFINITY;
+    const uint16_t* at = p.bounds + ((long long)page * c.kv_heads + r.h) * 2 * c.dim;
+    double score = 0.0;
+    for (int d = threadIdx.x & 31; d < c.dim; d += 32) {
+        const uint16_t* q = p.query + r.t * p.query_st[0] + (long long)r.h * p.group * p.query_st[1] + d;
+        double n = 0.0, s = 0.0;
         for (int g = 0; g < p.group; ++g, q += p.query_st[1]) {
-            const uint4 w = *reinterpret_cast<const uint4*>(q);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            const double x = widen16<BF16>(*q);
+            n += x < 0.0 ? x : 0.0;
+            s += x < 0.0 ? 0.0 : x;      // (NaN stays)
+        }
+        score += n * (double)widen16<BF16>(at[d]) + s * (double)widen16<BF16>(at[c.dim + d]);
+    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double x = widen16<BF16>(i & 1 ? words[i / 2] >> 16 : words[i / 2] & 0xffffu);
-                part[i] += (low ? x < 0.0 : !(x < 0.0)) ? x : 0.0;      // (NaN stays)
+    for (int o = 16; o > 0; o >>= 1) score += __shfl_xor_sync(0xffffffffu, score, o);
+    return score;
+}
+
+// ---- who chooses for a row: a block, or a warp.  A thread holds the keys of E consecutive pages (a block goes over more than
+// NT E pages in tiles, reading the scores again); key 0 is a page that does not compete.
+
+// (`scores` has places for a multiple of four pages)
+template <int E>
+__device__ __forceinline__ void load_keys(const Row& r, const float* scores, int first, uint32_t (&keys)[E]) {
+#pragma unroll
+    for (int j = 0; j < E; j += 4) {
+        const int i = first + j;
+        const float4 q = i < r.pages ? *reinterpret_cast<const float4*>(scores + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        keys[j] = i >= r.lo && i < r.hi ? key_of(q.x) : 0u;
+        keys[j + 1] = i + 1 >= r.lo && i + 1 < r.hi ? key_of(q.y) : 0u;
+        keys[j + 2] = i + 2 >= r.lo && i + 2 < r.hi ? key_of(q.z) : 0u;
+        keys[j + 3] = i + 3 >= r.lo && i + 3 < r.hi ? key_of(q.w) : 0u;
+    }
+}
+
+template <int NT, int E>
+struct BlockTeam {
+    static constexpr int SIZE = NT, RUN = E, BINS = 512;
+    const float* scores;
+    uint32_t* bins;              // shared: [BINS]
+    uint32_t* room;              // shared: [2][3 * NT / 32]
+    int turn = 0;
+    uint32_t keys[E];
+    __device__ int rank() const { return threadIdx.x; }
+    __device__ void sync() const { __syncthreads(); }
+    __device__ void load(const Row& r, int base) {
+        load_keys<E>(r, scores, base + rank() * E, keys);
+    }
+    // f(first page of this thread's run), for every tile of the row, by all threads
+    template <typename F>
+    __device__ void tiles(const Row& r, F f) {
+        for (int base = 0; base < r.pages; base += NT * E) {
+            if (r.pages > NT * E) load(r, base);
+            f(base + rank() * E);
+        }
+    }
+    template <typename Op>
+    __device__ void reduce(uint32_t (&v)[3], Op op) {
+        uint32_t* mine = room + (turn ^= 1) * (3 * NT / 32);      // (two rooms: one barrier is enough)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) v[j] = op.warp(v[j]);
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) mine[j * (NT / 32) + (threadIdx.x >> 5)] = v[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            v[j] = mine[j * (NT / 32)];
+#pragma unroll
+            for (int w = 1; w < NT / 32; ++w) v[j] = op(v[j], mine[j * (NT / 32) + w]);
+        }
+    }
+    // the sum of `n` over the threads before this one, and over all
+    __device__ uint32_t before(uint32_t n, uint32_t& total) {
+        uint32_t* mine = room + (turn ^= 1) * (3 * NT / 32);
+        const uint32_t upto = warp_upto(n);
+        if ((threadIdx.x & 31) == 31) mine[threadIdx.x >> 5] = upto;
+        __syncthreads();
+        uint32_t sum = upto - n;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) {
+            if (w < (int)(threadIdx.x >> 5)) sum += mine[w];
+            total += mine[w];
+        }
+        return sum;
+    }
+    __device__ static uint32_t warp_upto(uint32_t n) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, n, o);
+            if ((int)(threadIdx.x & 31) >= o) n += up;
+        }
+        return n;
+    }
+};
+
+template <int E>
+struct WarpTeam {
+    static constexpr int SIZE = 32, RUN = E, BINS = 256;
+    const float* scores;
+    uint32_t* bins;              // shared: [BINS], the warp's own
+    uint32_t keys[E];
+    __device__ int rank() const { return threadIdx.x & 31; }
+    __device__ void sync() const { __syncwarp(); }
+    __device__ void load(const Row& r, int) {
+        load_keys<E>(r, scores, rank() * E, keys);
+    }
+    template <typename F>
+    __device__ void tiles(const Row&, F f) { f(rank() * E); }
+    template <typename Op>
+    __device__ void reduce(uint32_t (&v)[3], Op op) const {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) v[j] = op.warp(v[j]);
+    }
+    __device__ uint32_t before(uint32_t n, uint32_t& total) const {
+        const uint32_t upto = BlockTeam<32, 1>::warp_upto(n);
+        total = __shfl_sync(0xffffffffu, upto, 31);
+        return upto - n;
+    }
+};
+
+struct Sum {
+    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return a + b; }
+    __device__ uint32_t warp(uint32_t v) const { return __reduce_add_sync(0xffffffffu, v); }
+};
+struct Largest {
+    __device__ uint32_t operator()(uint32_t a, uint32_t b) const { return max(a, b); }
+    __device__ uint32_t warp(uint32_t v) const { return __reduce_max_sync(0xffffffffu, v); }
+};
+
+// The `need`-th largest key of a row, or a key that as many as `need` reach: then `clean` is set.  Keys are in low .. high, more
+// than `need` of them.  A histogram over the range, and again over the bin that holds the place, until a bin is wanted whole.
+template <typename Team>
+__device__ uint32_t kth_key(const Row& r, Team& team, uint32_t need, uint32_t low, uint32_t high, bool& clean) {
+    constexpr int BINS = Team::BINS, PER = BINS / 32;
+    const int lane = threadIdx.x & 31;
+    while (true) {
+        const int width = 32 - __clz(high - low);      // bits of the range
+        const int shift = max(0, width - (31 - __clz(BINS)));
+        team.sync();                                   // (the bins of the round before have been read)
+        for (int i = team.rank(); i < BINS; i += Team::SIZE) team.bins[i] = 0;
+        team.sync();
+        team.tiles(r, [&](int) {
+#pragma unroll
+            for (int j = 0; j < Team::RUN; ++j)
+                if (team.keys[j] >= low && team.keys[j] <= high && team.keys[j])
+                    atomicAdd(&team.bins[(team.keys[j] - low) >> shift], 1u);
+        });
+        team.sync();
+        // every warp for itself: lane i has the i-th run of bins from the top
+        uint32_t n[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>(&team.bins[BINS - PER * (lane + 1) + i]);
+            n[i] = q.x, n[i + 1] = q.y, n[i + 2] = q.z, n[i + 3] = q.w;
+            sum += q.x + q.y + q.z + q.w;
+        }
+        const uint32_t upto = BlockTeam<32, 1>::warp_upto(sum);
+        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+        uint32_t above = upto - sum, bin = 0, count = 0;
+        if (lane == owner) {
+            bool open = true;
+#pragma unroll
+            for (int i = PER - 1; i >= 0; --i) {
+                if (open && above + n[i] >= need) {
+                    open = false;
+                    bin = BINS - PER * (lane + 1) + i;
+                    count = n[i];
+                }
+                if (open) above += n[i];
+            }
+        }
+        above = __shfl_sync(0xffffffffu, above, owner);
+        bin = __shfl_sync(0xffffffffu, bin, owner);
+        count = __shfl_sync(0xffffffffu, count, owner);
+        need -= above;
+        low += bin << shift;
+        clean = count == need;
+        if (clean || shift == 0) return low;
+        high = low + ((1u << shift) - 1);
+    }
+}
+
+// The same over 64-bit keys in low .. high - 1 that `each` goes over, three guesses at a time.
+template <typename Team, typename Each>
+__device__ unsigned long long kth_wide_key(Team& team, uint32_t need, unsigned long long low, unsigned long long high, bool& clean,
+                                           Each each) {
+    clean = false;
+    while (high - low > 1) {
+        const unsigned long long d = high - low, quarter = d / 4;
+        const unsigned long long m1 = low + (quarter > 0 ? quarter : 1), m2 = low + d / 2, m3 = low + (quarter > 0 ? 3 * quarter : 1);
+        uint32_t n[3] = {0, 0, 0};
+        each([&](unsigned long long key) {
+            n[0] += key >= m1;
+            n[1] += key >= m2;
+            n[2] += key >= m3;
+        });
+        team.reduce(n, Sum());
+        if (n[0] == need || n[1] == need || n[2] == need) {
+            clean = true;
+            return n[2] == need ? m3 : n[1] == need ? m2 : m1;
+        }
+        if (n[2] > need) low = m3;
+        else if (n[1] > need) low = m2, high = m3;
+        else if (n[0] > need) low = m1, high = m2;
+        else high = m1;
+    }
+    return low;
+}
+
+// Chooses the pages of a row and writes them.  `error`: E.  `exact`: the row's memory for sums in 64 bits.
+template <bool BF16, typename Team>
+__device__ void choose(const SelectParams& p, const Row& r, Team& team, float error, double* exact, int* out) {
+    constexpr int E = Team::RUN;
+    uint32_t(&keys)[E] = team.keys;
+    team.load(r, 0);
+    // keys above `sure` are chosen, keys from `open` on may be
+    uint32_t sure = 0xffffffffu, open = 0xffffffffu;
+    unsigned long long bar = ~0ull;       // of the latter: 64-bit keys above `bar`, and the first `equal` at it
+    uint32_t equal = 0;
+    if (r.need > 0) {
+        uint32_t ends[3] = {0, 0, 0};     // the largest key, the complement of the smallest
+        team.tiles(r, [&](int) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                ends[0] = max(ends[0], keys[j]);
+                if (keys[j]) ends[1] = max(ends[1], ~keys[j]);
+            }
+        });
+        team.reduce(ends, Largest());
+        bool clean;
+        uint32_t kth = kth_key(r, team, r.need, ~ends[1], ends[0], clean);
+        bool apart = false;
+        if (clean) {                      // the smallest above, the largest below
+            uint32_t near[3] = {0, 0, 0};
+            team.tiles(r, [&](int) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    if (keys[j] >= kth) near[0] = max(near[0], ~keys[j]);
+                    else near[1] = max(near[1], keys[j]);
+                }
+            });
+            team.reduce(near, Largest());
+            const uint32_t above = ~near[0];
+            apart = value_of(above) - value_of(near[1]) > 2.5f * error;
+            if (apart) sure = above - 1;
+            kth = above;
+        }
+        if (!apart) {
+            // (2.5: the sums below are rounded, too)
+            const float t = value_of(kth);
+            const bool known = error < INFINITY;
+            sure = known ? key_of(t + 2.5f * error) : 0xffffffffu;
+            open = known ? key_of(t - 2.5f * error) : 1u;
+            uint32_t n[3] = {0, 0, 0};
+            team.tiles(r, [&](int) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    n[0] += keys[j] > sure;
+                    n[1] += keys[j] >= open && keys[j] <= sure;
+                }
+            });
+            team.reduce(n, Sum());
+            const uint32_t left = r.need - n[0];
+            if (n[1] == left) {           // all of them
+                bar = 0;
+            } else {
+                team.tiles(r, [&](int i) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        uint32_t todo = __ballot_sync(0xffffffffu, keys[j] >= open && keys[j] <= sure);
+                        while (todo) {
+                            const int src = __ffs(todo) - 1;
+                            todo &= todo - 1;
+                            const int page = __shfl_sync(0xffffffffu, i, src) + j;
+                            const double s = exact_score<BF16>(p, r, page);
+                            if ((int)(threadIdx.x & 31) == src) exact[page] = s;
+                        }
+                    }
+                });
+                team.sync();
+                auto over_open = [&](auto count) {
+                    team.tiles(r, [&](int i) {
+#pragma unroll
+                        for (int j = 0; j < E; ++j)
+                            if (keys[j] >= open && keys[j] <= sure) count(key_of(exact[i + j]));
+                    });
+                };
+                // (within E of sums that are within 2.5 E of t)
+                bar = kth_wide_key(team, left, known ? key_of((double)t - 4.0 * error) : 0ull,
+                                   known ? key_of((double)t + 4.0 * error) + 1 : ~0ull, clean, over_open);
+                if (clean) {
+                    bar -= 1;
+                } else {
+                    uint32_t above[3] = {0, 0, 0};
+                    over_open([&](unsigned long long key) { above[0] += key > bar; });
+                    team.reduce(above, Sum());
+                    equal = left - above[0];
+                }
             }
         }
     }
-    double* out = p.scores + ((long long)blockIdx.z * c.kv_heads + h) * c.width;
-    const int at_once = 32 / span;
-    for (int i = 0; i < SCORE_PAGES / 8; i += at_once) {
-        const int page = base + i + lane / span;
-        const bool take = page < seen && page < base + SCORE_PAGES / 8;
-        const int at = take ? physical_page(c, b, page) : -1;
-        double score = 0.0;
-        if (at >= 0 && v < vectors) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p.bounds + ((long long)at * c.kv_heads + h) * 2 * D + v * 8);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    uint32_t place = 0, equal_before = 0, total;
+    team.tiles(r, [&](int i) {
+        uint32_t taken = 0, same = 0;     // a bit per page of the run
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                score += part[e] * (double)widen16<BF16>(e & 1 ? words[e / 2] >> 16 : words[e / 2] & 0xffffu);
+        for (int j = 0; j < E; ++j) {
+            bool take = i + j < r.pages && (keys[j] == 0 || keys[j] > sure);
+            if (keys[j] >= open && keys[j] <= sure) {
+                const unsigned long long wide = bar == 0 ? 1ull : key_of(exact[i + j]);
+                take = wide > bar;
+                if (wide == bar) same |= 1u << j;
+            }
+            if (take) taken |= 1u << j;
         }
-        for (int o = span / 2; o > 0; o >>= 1) score += __shfl_xor_sync(0xffffffffu, score, o);
-        if (take && v == 0) out[page] = at < 0 ? -INFINITY : score != score ? INFINITY : score;
-    }
+        if (equal > 0) {                  // (the same for all)
+            uint32_t rank = equal_before + team.before(__popc(same), total);
+            equal_before += total;
+            for (; same && rank < equal; ++rank, same &= same - 1) taken |= same & -same;
+        }
+        uint32_t at = place + team.before(__popc(taken), total);
+        for (; taken; ++at, taken &= taken - 1)
+            if (at < (uint32_t)p.k) out[at] = i + __ffs(taken) - 1;
+        place += total;
+    });
+    for (int i = (int)place + team.rank(); i < p.k; i += Team::SIZE) out[i] = -1;
 }
 
-// Larger score, larger key.
-__device__ __forceinline__ unsigned long long key_of_score(double s) {
-    const long long bits = __double_as_longlong(s == 0.0 ? 0.0 : s);     // (zeros of both signs are equal)
-    return bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | 0x8000000000000000ull;
+// The rows that need no scores: behind the last sequence, or with no more pages than are asked for.
+__device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row& r, int* out, int rank, int size) {
+    if (b >= p.c.sequences) {
+        if (p.fill_tail)
+            for (int i = rank; i < p.k; i += size) out[i] = -1;
+        return true;
+    }
+    if (r.pages > p.k) return false;
+    for (int i = rank; i < p.k; i += size) out[i] = i < r.pages ? i : -1;
+    return true;
 }
 
-constexpr int CHOOSE_THREADS = 256;
-constexpr int DIGIT_BITS = 11, DIGITS = 1 << DIGIT_BITS;
+// ------------------------------------------------------------------ few tokens a sequence
+constexpr int ROW_THREADS = 256;
+typedef BlockTeam<ROW_THREADS, 8> RowTeam;
 
-// Exclusive scan of one count per thread; `total` is the block's.
-__device__ __forceinline__ uint32_t scan_block(uint32_t v, uint32_t* warp_sums, uint32_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = inc;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < CHOOSE_THREADS / 32; ++w) {
-        if (w < warp) before += warp_sums[w];
-        total += warp_sums[w];
-    }
-    return before + inc - v;
-}
-
-// A CTA per (token, kv head): radix selection over the 64-bit keys of the scores, 11 bits at a time from the top.
-__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_constant__ SelectParams p) {
-    __shared__ uint32_t bins[DIGITS];
-    __shared__ uint32_t warp_sums[CHOOSE_THREADS / 32];
-    __shared__ uint32_t found[3];
+// grid: (CL * tokens, kv heads); shared memory: `pitch` scores.  A warp takes 16 pages at a time as the rows of a matrix
+// instruction straight from memory -- a lane loads eight neighbouring features, which serve as those that the instruction wants of
+// it, in the order that the parts are given in as well.  The parts' two pieces are two of its eight columns.
+template <bool BF16, int DP, int CL>
+__global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int CHUNKS = DP / 16;               // 32 of the 2 D features
+    extern __shared__ __align__(16) float row_scores[];
+    __shared__ float reach_of_cta[CL];
+    __shared__ float warp_reach[ROW_THREADS / 32], warp_size[ROW_THREADS / 32];
+    __shared__ uint32_t room[2 * 3 * ROW_THREADS / 32];
+    __shared__ __align__(16) uint32_t bins[RowTeam::BINS];
+    __shared__ __align__(16) uint16_t parts[3][2 * DP];       // what 16 bits hold, the rest, zeros
+    if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     grid_dependency_wait();
     grid_launch_dependents();
     const Batch& c = p.c;
-    const int tid = threadIdx.x, h = blockIdx.x, t = p.t0 + (int)blockIdx.y;
-    int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
+    const int D = c.dim, h = blockIdx.y, rank = (int)(blockIdx.x % CL), t = p.t0 + (int)(blockIdx.x / CL);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = sequence_of(c, t);
-    if (b >= c.sequences) {
-        if (p.fill_tail)
-            for (int i = tid; i < p.k; i += CHOOSE_THREADS) out[i] = -1;
-        return;
-    }
-    const long long seen = pages_seen(c, position_of(c, b, t));
-    const int pages = (int)min(seen, (long long)c.width);
-    if (pages <= p.k) {
-        for (int i = tid; i < p.k; i += CHOOSE_THREADS) out[i] = i < pages ? i : -1;
-        return;
-    }
-    const int lo = min(p.first, pages), hi = (int)max((long long)lo, min((long long)pages, seen - p.last));   // candidates
-    uint32_t need = (uint32_t)max(0, p.k - lo - (pages - hi));
-    const double* scores = p.scores + ((long long)blockIdx.y * c.kv_heads + h) * c.width;
+    const long long pos = b < c.sequences ? position_of(c, b, t) : -1;
 
-    // the smallest key chosen, as a prefix of `bits` bits; `need`: how many with exactly that prefix
-    unsigned long long prefix = 0;
-    int bits = 0;
-    uint32_t equal = (uint32_t)(hi - lo);
-    while (need < equal && need > 0 && bits < 64) {
-        const int width = min(DIGIT_BITS, 64 - bits), shift = 64 - bits - width;
-        __syncthreads();
-        for (int i = tid; i < DIGITS; i += CHOOSE_THREADS) bins[i] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += CHOOSE_THREADS) {
-            const unsigned long long key = key_of_score(scores[i]);
-            if (bits == 0 || key >> (64 - bits) == prefix) atomicAdd(&bins[(uint32_t)(key >> shift) & ((1u << width) - 1)], 1u);
+    // a thread has one of the 2 D parts: the first D meet the lows, the others the highs
+    if (tid < 2 * DP) {
+        float part = 0.f;
+        if (tid < 2 * D && b < c.sequences) {
+            const bool low = tid < D;
+            const uint16_t* q = p.query + t * p.query_st[0] + (long long)h * p.group * p.query_st[1] + (low ? tid : tid - D);
+#pragma unroll 4
+            for (int g = 0; g < p.group; ++g) {
+                const float x = widen16<BF16>(q[g * p.query_st[1]]);
+                part += (low ? x < 0.f : !(x < 0.f)) ? x : 0.f;      // (NaN stays)
+            }
         }
-        __syncthreads();
-        // from the top: thread i sums the bins of one run
-        constexpr int RUN = DIGITS / CHOOSE_THREADS;
-        const int top = DIGITS - 1 - tid * RUN;
-        uint32_t sum = 0;
+        float rest, z;
+        parts[0][tid] = (uint16_t)round_pair<BF16>(part, 0.f, rest, z);
+        parts[1][tid] = (uint16_t)round_pair<BF16>(rest, 0.f, z, z);
+        parts[2][tid] = 0;
+        float size = fabsf(part);
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) sum += bins[top - i];
-        uint32_t total;
-        uint32_t above = scan_block(sum, warp_sums, total);
-        if (above < need && need <= above + sum) {
-            int bin = top;
-            while (above + bins[bin] < need) above += bins[bin--];
-            found[0] = (uint32_t)bin;
-            found[1] = need - above;
-            found[2] = bins[bin];
+        for (int o = 16; o > 0; o >>= 1) size += __shfl_xor_sync(0xffffffffu, size, o);
+        if (lane == 0) warp_size[warp] = size;
+    } else if (lane == 0) {
+        warp_size[warp] = 0.f;
+    }
+    Row r = {};
+    if (b < c.sequences) r.set(p, t, h, b, pos);
+    int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
+    if (b >= c.sequences || r.pages <= p.k) {       // (all CTAs of the cluster)
+        if (rank == 0) settled(p, b, r, out, tid, ROW_THREADS);
+        if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        return;
+    }
+    const int per = (r.hi - r.lo + CL - 1) / CL, begin = r.lo + rank * per, end = min(r.hi, begin + per);
+    const int* table = c.table + b * c.table_ld;
+    int base = begin + warp * 16;
+    int entry = base + (lane & 15) < end ? table[base + (lane & 15)] : -1;
+    uint32_t high_bits = 0, low_bits = 0x80008000u;       // the largest bit patterns, as unsigned and as signed
+    bool lacking = false;
+    __syncthreads();
+    if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // the first CTA is there
+    uint32_t to = smem_u32(row_scores);
+    if constexpr (CL > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(to), "r"(0));
+    const int row = lane >> 2, col = lane & 3;
+    const uint16_t* columns = parts[min(row, 2)] + col * 8;
+    while (base < end) {
+        const int page0 = __shfl_sync(0xffffffffu, entry, row), page1 = __shfl_sync(0xffffffffu, entry, row + 8);
+        const bool there0 = page0 >= 0 && page0 < c.pages, there1 = page1 >= 0 && page1 < c.pages;
+        const uint16_t* at0 = p.bounds + ((long long)(there0 ? page0 : 0) * c.kv_heads + h) * 2 * D + col * 8;
+        const uint16_t* at1 = p.bounds + ((long long)(there1 ? page1 : 0) * c.kv_heads + h) * 2 * D + col * 8;
+        const int next = base + ROW_THREADS / 32 * 16;
+        entry = next + (lane & 15) < end ? table[next + (lane & 15)] : -1;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s0 = 0; s0 < CHUNKS; s0 += 4) {
+            uint4 w0[4], w1[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bool in = (s0 + s) * 32 + col * 8 < 2 * D;
+                w0[s] = there0 && in ? *reinterpret_cast<const uint4*>(at0 + (s0 + s) * 32) : make_uint4(0, 0, 0, 0);
+                w1[s] = there1 && in ? *reinterpret_cast<const uint4*>(at1 + (s0 + s) * 32) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const uint4 f = *reinterpret_cast<const uint4*>(columns + (s0 + s) * 32);
+                // (every step starts from zero: see score_error)
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint32_t a0[4] = {w0[s].x, w1[s].x, w0[s].y, w1[s].y}, a1[4] = {w0[s].z, w1[s].z, w0[s].w, w1[s].w};
+                mma16816<BF16>(x, a0, f.x, f.y);
+                mma16816<BF16>(y, a1, f.z, f.w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += x[i] + y[i];
+                high_bits = __vimax3_u16x2(high_bits, w0[s].x, w0[s].y);
+                high_bits = __vimax3_u16x2(high_bits, w0[s].z, w0[s].w);
+                high_bits = __vimax3_u16x2(high_bits, w1[s].x, w1[s].y);
+                high_bits = __vimax3_u16x2(high_bits, w1[s].z, w1[s].w);
+                low_bits = __vimax3_s16x2(low_bits, w0[s].x, w0[s].y);
+                low_bits = __vimax3_s16x2(low_bits, w0[s].z, w0[s].w);
+                low_bits = __vimax3_s16x2(low_bits, w1[s].x, w1[s].y);
+                low_bits = __vimax3_s16x2(low_bits, w1[s].z, w1[s].w);
+            }
+        }
+        if (col < 2) {          // column 0 and 1 together are the score; lane 4 i has page i's and page i + 8's
+            const int i = base + row + 8 * col;
+            const float other = __shfl_sync(0x33333333u, acc[2] + acc[3], lane & ~1);
+            const float score = col == 0 ? acc[0] + acc[1] : other;
+            const bool there = col == 0 ? there0 : there1;
+            if (i < end) {
+                lacking |= !there;
+                const float s = there ? score : -INFINITY;
+                if constexpr (CL > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(s) : "memory");
+                else row_scores[i] = s;
+            }
+        }
+        __syncwarp();
+        base = next;
+    }
+    if (lacking) report(c, FCS_STATUS_BAD_PAGE);
+    float most = reach_of<BF16>(high_bits, low_bits);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) warp_reach[warp] = most;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 0; w < ROW_THREADS / 32; ++w) most = max_or_nan(most, warp_reach[w]);
+        if constexpr (CL > 1) {
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&reach_of_cta[rank])), "r"(0));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(most) : "memory");
+        } else {
+            reach_of_cta[0] = most;
+        }
+    }
+    if constexpr (CL > 1) {
+        __syncwarp();
+        cluster_sync();
+        if (rank > 0) return;
+    } else {
+        __syncthreads();
+    }
+    most = reach_of_cta[0];
+    for (int i = 1; i < CL; ++i) most = max_or_nan(most, reach_of_cta[i]);
+    float size = 0.f;
+    for (int w = 0; w < ROW_THREADS / 32; ++w) size += warp_size[w];
+    RowTeam team{row_scores, bins, room};
+    choose<BF16>(p, r, team, score_error<BF16>(p, size, most), p.exact + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch, out);
+}
+
+// ------------------------------------------------------------------ many tokens a sequence
+constexpr int TILE_TOKENS = 64, TILE_PAGES = 64;
+constexpr int TILES_THREADS = 256;
+
+inline int tiles_row_bytes(int dim) { return 4 * dim + 16; }     // of a row of 2 D values in shared memory: no bank twice
+inline int tiles_smem(int dim) { return 3 * 64 * tiles_row_bytes(dim); }
+
+// 64 tokens of one sequence, a share of the pages that they see.  grid: (token tiles, kv heads, splits); sequence b has the
+// tiles from starts[b] / 64 + b on, at least as many as it needs.
+template <bool BF16>
+__global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid_constant__ SelectParams p) {
+    extern __shared__ __align__(16) uint8_t tiles_smem_raw[];
+    __shared__ uint32_t reach_of_warp[TILES_THREADS / 32];
+    __shared__ float size_of_token[TILE_TOKENS];
+    __shared__ uint8_t missing[TILE_PAGES];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Batch& c = p.c;
+    const int D = c.dim, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long tile_id = (long long)blockIdx.x + max(0, p.t0 / TILE_TOKENS - 1);
+    int b = 0;
+    for (int base = 0; base < c.sequences; base += TILES_THREADS) {
+        const int i = base + tid + 1;
+        b += __syncthreads_count(i <= c.sequences && (c.starts[i] / TILE_TOKENS) + (long long)i <= tile_id);
+    }
+    if (b >= c.sequences) return;
+    const long long s0 = c.starts[b], s1 = c.starts[b + 1];
+    const long long first = s0 + (tile_id - (s0 / TILE_TOKENS + b)) * TILE_TOKENS;
+    if (s0 < 0 || s1 > c.tokens || first < s0 || first >= s1) return;
+    if (first >= p.t1 || first + TILE_TOKENS <= p.t0) return;
+    const int tokens = (int)min((long long)TILE_TOKENS, s1 - first), t_first = (int)first;
+    // pages that the last token lets compete, cut over the splits in whole tiles
+    const long long seen = pages_seen(c, position_of(c, b, t_first + tokens - 1));
+    const int pages = (int)max(0ll, min((long long)c.width, seen - p.last));
+    const int page_tiles = (pages + TILE_PAGES - 1) / TILE_PAGES, per = (page_tiles + p.splits - 1) / p.splits;
+    const int begin = blockIdx.z * per * TILE_PAGES, end = min(pages, begin + per * TILE_PAGES);
+
+    const int row_bytes = 4 * D + 16;
+    uint8_t* const hi = tiles_smem_raw;                  // [tokens][2 D]: n and p, what 16 bits hold of them
+    uint8_t* const lo = hi + TILE_TOKENS * row_bytes;    // the rest
+    uint8_t* const tile = lo + TILE_TOKENS * row_bytes;  // [pages][2 D]
+    const int my_row = tid >> 2, my_vec = tid & 3;       // four threads a row
+    {
+        float size = 0.f;
+        for (int v = my_vec; v < D / 8; v += 4) {
+            float n[8], s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n[i] = s[i] = 0.f;
+            if (my_row < tokens) {
+                const uint16_t* q = p.query + (t_first + my_row) * p.query_st[0] + (long long)h * p.group * p.query_st[1] + v * 8;
+                for (int g = 0; g < p.group; ++g, q += p.query_st[1]) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(q);
+                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 x = widen_pair<BF16>(words[i]);
+                        n[2 * i] += x.x < 0.f ? x.x : 0.f;
+                        n[2 * i + 1] += x.y < 0.f ? x.y : 0.f;
+                        s[2 * i] += x.x < 0.f ? 0.f : x.x;
+                        s[2 * i + 1] += x.y < 0.f ? 0.f : x.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) size += s[i] - n[i];
+            uint32_t nh[4], nl[4], sh[4], sl[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float ra, rb, z;
+                nh[i] = round_pair<BF16>(n[2 * i], n[2 * i + 1], ra, rb);
+                nl[i] = round_pair<BF16>(ra, rb, z, z);
+                sh[i] = round_pair<BF16>(s[2 * i], s[2 * i + 1], ra, rb);
+                sl[i] = round_pair<BF16>(ra, rb, z, z);
+            }
+            const int at = my_row * row_bytes + v * 16;
+            *reinterpret_cast<uint4*>(hi + at) = make_uint4(nh[0], nh[1], nh[2], nh[3]);
+            *reinterpret_cast<uint4*>(lo + at) = make_uint4(nl[0], nl[1], nl[2], nl[3]);
+            *reinterpret_cast<uint4*>(hi + at + 2 * D) = make_uint4(sh[0], sh[1], sh[2], sh[3]);
+            *reinterpret_cast<uint4*>(lo + at + 2 * D) = make_uint4(sl[0], sl[1], sl[2], sl[3]);
+        }
+        size += __shfl_xor_sync(0xffffffffu, size, 1);
+        size += __shfl_xor_sync(0xffffffffu, size, 2);
+        if (my_vec == 0) size_of_token[my_row] = size;
+    }
+
+    const int wm = warp & 3, wn = warp >> 2;
+    const uint32_t a_at = smem_u32(hi) + (wm * 16 + (lane & 15)) * row_bytes + (lane >> 4) * 16;
+    const uint32_t lo_off = TILE_TOKENS * row_bytes;
+    const uint32_t b_at = smem_u32(tile) + (wn * 32 + (lane & 7) + (lane >> 4) * 8) * row_bytes + ((lane >> 3) & 1) * 16;
+    uint32_t high_bits = 0, low_bits = 0x80008000u;       // the largest bit patterns, as unsigned and as signed
+    uint4 next[8];
+    int next_page = -1;
+    auto fetch = [&](int base) {        // this thread's pieces of its page of the tile at `base`
+        next_page = base + my_row < end ? physical_page(c, b, base + my_row) : -1;
+        const uint16_t* at = p.bounds + ((long long)max(next_page, 0) * c.kv_heads + h) * 2 * D;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int v = my_vec + 4 * j;
+            next[j] = next_page >= 0 && v < D / 4 ? *reinterpret_cast<const uint4*>(at + v * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (begin < end) fetch(begin);
+    for (int base = begin; base < end; base += TILE_PAGES) {
+        __syncthreads();                // the tile before has been read
+        if (my_vec == 0) missing[my_row] = next_page < 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int v = my_vec + 4 * j;
+            if (v < D / 4) *reinterpret_cast<uint4*>(tile + my_row * row_bytes + v * 16) = next[j];
+            high_bits = __vimax3_u16x2(__vimax3_u16x2(high_bits, next[j].x, next[j].y), next[j].z, next[j].w);
+            low_bits = __vimax3_s16x2(__vimax3_s16x2(low_bits, next[j].x, next[j].y), next[j].z, next[j].w);
         }
         __syncthreads();
-        prefix = prefix << width | found[0];
-        need = found[1];
-        equal = found[2];
-        bits += width;
-    }
-    // chosen: the forced ones, keys above the prefix, and of those with the prefix the first `need`
-    uint32_t place = 0, equal_before = 0;
-    for (int i0 = 0; i0 < pages; i0 += CHOOSE_THREADS) {
-        const int i = i0 + tid;
-        bool take = i < pages && (i < lo || i >= hi), same = false;
-        if (i >= lo && i < hi && need > 0) {
-            const unsigned long long key = bits == 0 ? 0ull : key_of_score(scores[i]) >> (64 - bits);
-            take = key > prefix;
-            same = key == prefix;
+        if (base + TILE_PAGES < end) fetch(base + TILE_PAGES);
+        float acc[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        // Every step starts from zero and is added up by ordinary additions: a tensor core drops what lies below the last
+        // bit of its largest term, and a running sum would be that term at every step.
+#pragma unroll 4
+        for (int k = 0; k < D / 8; ++k) {       // 16 of the 2 D terms
+            uint32_t ah[4], al[4], b0[4], b1[4];
+            ldmatrix_x4(a_at + k * 32, ah);
+            ldmatrix_x4(a_at + lo_off + k * 32, al);
+            ldmatrix_x4(b_at + k * 32, b0);
+            ldmatrix_x4(b_at + 16 * row_bytes + k * 32, b1);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t* f = n < 2 ? b0 : b1;
+                float step[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816<BF16>(step, al, f[2 * (n & 1)], f[2 * (n & 1) + 1]);
+                mma16816<BF16>(step, ah, f[2 * (n & 1)], f[2 * (n & 1) + 1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][i] += step[i];
+            }
         }
-        uint32_t total;
-        const uint32_t rank = equal_before + scan_block(same, warp_sums, total);
-        equal_before += total;
-        if (same && rank < need) take = true;
-        const uint32_t at = place + scan_block(take, warp_sums, total);
-        if (take && at < (uint32_t)p.k) out[at] = i;
-        place += total;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int col = wn * 32 + n * 8 + (lane & 3) * 2, page = base + col;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = wm * 16 + (lane >> 2) + 8 * half, t = t_first + row;
+                if (row < tokens && t >= p.t0 && t < p.t1 && page < end)      // (the pitch is even: the second of a pair has a place)
+                    *reinterpret_cast<float2*>(p.scores + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch + page) =
+                        make_float2(missing[col] ? -INFINITY : acc[n][2 * half], missing[col + 1] ? -INFINITY : acc[n][2 * half + 1]);
+            }
+        }
     }
-    for (int i = (int)place + tid; i < p.k; i += CHOOSE_THREADS) out[i] = -1;
+    float most = reach_of<BF16>(high_bits, low_bits);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) reach_of_warp[warp] = __float_as_uint(most);
+    __syncthreads();
+    if (tid < tokens && t_first + tid >= p.t0 && t_first + tid < p.t1) {
+        for (int w = 0; w < TILES_THREADS / 32; ++w) most = max_or_nan(most, __uint_as_float(reach_of_warp[w]));
+        p.errors[((long long)(t_first + tid - p.t0) * c.kv_heads + h) * p.splits + blockIdx.z] =
+            score_error<BF16>(p, size_of_token[tid], most);
+    }
+}
+
+constexpr int CHOOSE_THREADS = 128;
+
+// A warp per row, of at most 32 E pages, or (E = 0) a block.
+template <bool BF16, int E>
+__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int ROWS = E > 0 ? CHOOSE_THREADS / 32 : 1;
+    typedef BlockTeam<CHOOSE_THREADS, 16> Block;
+    typedef WarpTeam<(E > 0 ? E : 4)> Warp;
+    __shared__ uint32_t room[2 * 3 * CHOOSE_THREADS / 32];
+    __shared__ __align__(16) uint32_t bins[E > 0 ? ROWS * Warp::BINS : Block::BINS];
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const Batch& c = p.c;
+    const long long row = (long long)blockIdx.x * ROWS + (E > 0 ? threadIdx.x >> 5 : 0);
+    const long long at = row / c.kv_heads;
+    const int h = (int)(row % c.kv_heads), t = p.t0 + (int)at;
+    if (at >= p.t1 - p.t0) return;
+    int b = 0;
+    if constexpr (E > 0) {
+        const int lane = threadIdx.x & 31;
+        for (int base = 0; base < c.sequences; base += 32)
+            b += __popc(__ballot_sync(0xffffffffu, base + lane < c.sequences && c.starts[base + lane + 1] <= t));
+    } else {
+        b = sequence_of(c, t);
+    }
+    Row r = {};
+    if (b < c.sequences) r.set(p, t, h, b, position_of(c, b, t));
+    int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
+    const float* scores = p.scores + row * p.pitch;
+    double* exact = p.exact + row * p.pitch;
+    if (settled(p, b, r, out, E > 0 ? threadIdx.x & 31 : threadIdx.x, E > 0 ? 32 : CHOOSE_THREADS)) return;
+    float error = 0.f;
+    for (int s = 0; s < p.splits; ++s) error = max_or_nan(error, p.errors[row * p.splits + s]);
+    if (!(error < INFINITY)) error = INFINITY;
+    if constexpr (E > 0) {
+        Warp team{scores, bins + (threadIdx.x >> 5) * Warp::BINS};
+        choose<BF16>(p, r, team, error, exact, out);
+    } else {
+        Block team{scores, bins, room};
+        choose<BF16>(p, r, team, error, exact, out);
+    }
 }
 
 }  // namespace paged

@@ -7,8 +7,8 @@
 #include "../../include/flash_colsum_b200.h"
 #include "host_common.h"
 #include "paged_append.cuh"
-#include "paged_select.cuh"
 #include "paged_attend.cuh"
+#include "paged_select.cuh"
 
 namespace fcs {
 namespace paged {
@@ -155,16 +155,127 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
 }
 
 // ------------------------------------------------------------------ select
-// Tokens whose scores are held at once: 256 MiB of them, and as many as a grid takes.
-static long long select_tokens_at_once(const FcsPagedCache* c) {
-    const long long row = 8ll * c->kv_heads * c->table_width;
-    long long n = (256ll << 20) / row;
-    n = n < 1 ? 1 : n > 32768 ? 32768 : n;
-    return n < c->tokens ? n : c->tokens;
+constexpr int ROW_PAGES = 51200;       // scores that a CTA's shared memory holds
+
+// Scores of a row, with a place behind the last.
+static long long select_pitch(const FcsPagedCache* c) { return (c->table_width + 4ll) & ~3ll; }
+// Many tokens a sequence: the scores of 64 tokens and 64 pages are worth a tile of their own from about eight on.
+static bool select_by_tiles(const FcsPagedCache* c) {
+    return c->starts && (c->tokens >= 8ll * c->sequences || select_pitch(c) > ROW_PAGES);
 }
 
-static size_t select_workspace(const FcsPagedCache* c) {
-    return (size_t)select_tokens_at_once(c) * c->kv_heads * c->table_width * 8;
+struct SelectPlan {
+    bool tiles;
+    long long pitch, at_once;      // tokens of a launch: 256 MiB of scratch, and as many as a grid takes
+    int splits;
+    size_t errors, scores, exact, bytes;     // offsets into the workspace
+};
+
+static SelectPlan select_plan(const FcsPagedCache* c) {
+    SelectPlan s;
+    s.tiles = select_by_tiles(c);
+    s.pitch = select_pitch(c);
+    const long long row = (s.tiles ? 12 : 8) * (long long)c->kv_heads * s.pitch;
+    s.at_once = (256ll << 20) / row;
+    s.at_once = s.at_once < 1 ? 1 : s.at_once > c->tokens ? c->tokens : s.at_once;
+    s.splits = 1;
+    if (s.tiles) {
+        const long long ctas = (s.at_once / TILE_TOKENS + 1) * c->kv_heads, most = (c->table_width + 2 * TILE_PAGES - 1) / (2 * TILE_PAGES);
+        while (s.splits < most && s.splits < 64 && ctas * s.splits < num_sms()) s.splits *= 2;
+    }
+    const long long rows = s.at_once * c->kv_heads;
+    s.exact = 0;
+    s.scores = s.exact + (size_t)rows * s.pitch * 8;
+    s.errors = s.scores + (s.tiles ? (size_t)rows * s.pitch * 4 : 0);
+    s.bytes = s.errors + (s.tiles ? (size_t)rows * s.splits * 4 : 0);
+    return s;
+}
+
+template <typename F>
+static cudaError_t allow_smem(F* kern, int bytes, bool wide_cluster = false) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && wide_cluster) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e;
+}
+
+// Runs `set_up` once per device and instance (`done` is the instance's).
+template <typename F>
+static cudaError_t once_per_device(bool (&done)[64], F set_up) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+    e = set_up();
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+    return e;
+}
+
+template <bool BF16, int DP, int CL>
+static cudaError_t launch_select_row(const SelectParams& p, unsigned tokens, cudaStream_t stream) {
+    static bool done[64] = {false};
+    const cudaError_t e = once_per_device(done, [] { return allow_smem(select_row_kernel<BF16, DP, CL>, ROW_PAGES * 4, CL > 8); });
+    if (e != cudaSuccess) return e;
+    return launch(select_row_kernel<BF16, DP, CL>, dim3(CL * tokens, p.c.kv_heads), ROW_THREADS, p.pitch * 4, CL, stream, p);
+}
+
+template <bool BF16, int DP>
+static cudaError_t launch_select_cl(int cl, const SelectParams& p, unsigned tokens, cudaStream_t stream) {
+    return cl == 16  ? launch_select_row<BF16, DP, 16>(p, tokens, stream)
+           : cl == 8 ? launch_select_row<BF16, DP, 8>(p, tokens, stream)
+           : cl == 4 ? launch_select_row<BF16, DP, 4>(p, tokens, stream)
+           : cl == 2 ? launch_select_row<BF16, DP, 2>(p, tokens, stream)
+                     : launch_select_row<BF16, DP, 1>(p, tokens, stream);
+}
+
+// Whether the current device can hold a cluster of sixteen CTAs of the row kernel (asked once per device).
+template <bool BF16>
+static bool clusters_of_sixteen_fit() {
+    static int known[64] = {0};         // 0: not asked, 1: no, 2: yes
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+    if (known[dev] == 0) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(16);
+        cfg.blockDim = dim3(ROW_THREADS);
+        cfg.dynamicSmemBytes = ROW_PAGES * 4;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 16;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        const bool fits = allow_smem(select_row_kernel<BF16, 128, 16>, ROW_PAGES * 4, true) == cudaSuccess &&
+                          cudaOccupancyMaxActiveClusters(&n, select_row_kernel<BF16, 128, 16>, &cfg) == cudaSuccess && n > 0;
+        if (!fits) cudaGetLastError();
+        known[dev] = fits ? 2 : 1;
+    }
+    return known[dev] == 2;
+}
+
+template <bool BF16>
+static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t stream) {
+    const unsigned tokens = (unsigned)(p.t1 - p.t0);
+    if (!tiles) {
+        // CTAs of a row: as many as the device runs at once, 64 pages for each at least
+        const long long rows = (long long)tokens * p.c.kv_heads;
+        int cl = 1;
+        const int widest = clusters_of_sixteen_fit<BF16>() ? 16 : 8;
+        while (cl < widest && rows * cl * 2 <= 4ll * num_sms() && p.c.width >= 128 * cl) cl *= 2;
+        return p.c.dim > 64 ? launch_select_cl<BF16, 128>(cl, p, tokens, stream) : launch_select_cl<BF16, 64>(cl, p, tokens, stream);
+    }
+    static bool done[64] = {false};
+    cudaError_t e = once_per_device(done, [] { return allow_smem(score_tiles_kernel<BF16>, tiles_smem(128)); });
+    if (e != cudaSuccess) return e;
+    const int first = p.t0 / TILE_TOKENS - 1 > 0 ? p.t0 / TILE_TOKENS - 1 : 0;
+    const dim3 grid((unsigned)((p.t1 - 1) / TILE_TOKENS - first + 1 + p.c.sequences), p.c.kv_heads, p.splits);
+    e = launch(score_tiles_kernel<BF16>, grid, TILES_THREADS, tiles_smem(p.c.dim), 1, stream, p);
+    if (e != cudaSuccess) return e;
+    const long long rows = (long long)tokens * p.c.kv_heads;
+    const unsigned by_warp = (unsigned)((rows + CHOOSE_THREADS / 32 - 1) / (CHOOSE_THREADS / 32));
+    return p.c.width <= 512    ? launch(choose_kernel<BF16, 16>, dim3(by_warp), CHOOSE_THREADS, 0, 1, stream, p)
+           : p.c.width <= 1024 ? launch(choose_kernel<BF16, 32>, dim3(by_warp), CHOOSE_THREADS, 0, 1, stream, p)
+                               : launch(choose_kernel<BF16, 0>, dim3((unsigned)rows), CHOOSE_THREADS, 0, 1, stream, p);
 }
 
 static int select(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const void* bounds,
@@ -181,9 +292,11 @@ static int select(const FcsPagedCache* cache, const void* query, const int64_t* 
     if (!chosen) return fail(FCS_ERR_INVALID_ARGUMENT, "chosen is NULL");
     if (k < 1 || first < 0 || last < 1 || (long long)first + last > k)
         return fail(FCS_ERR_INVALID_ARGUMENT, "k must hold the first and the last pages (k=%d first=%d last=%d)", k, first, last);
-    const size_t need = select_workspace(cache);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)
-        return fail(FCS_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes, got %zu", need, workspace_bytes);
+    const SelectPlan plan = select_plan(cache);
+    if (!plan.tiles && plan.pitch > ROW_PAGES)
+        return fail(FCS_ERR_UNSUPPORTED, "one token a sequence chooses from at most %d pages, got %d", ROW_PAGES - 4, cache->table_width);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes)
+        return fail(FCS_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes, got %zu", plan.bytes, workspace_bytes);
     p.query = static_cast<const uint16_t*>(query);
     p.bounds = static_cast<const uint16_t*>(bounds);
     p.query_st[0] = query_stride[0];
@@ -193,16 +306,17 @@ static int select(const FcsPagedCache* cache, const void* query, const int64_t* 
     p.first = first;
     p.last = last;
     p.chosen = chosen;
-    p.scores = static_cast<double*>(workspace);
+    p.exact = reinterpret_cast<double*>(static_cast<char*>(workspace) + plan.exact);
+    p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.scores);
+    p.errors = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.errors);
+    p.pitch = (int)plan.pitch;
+    p.splits = plan.splits;
     p.fill_tail = fill_tail;
-    const long long at_once = select_tokens_at_once(cache);
-    for (long long t0 = 0; t0 < cache->tokens; t0 += at_once) {
-        const unsigned n = (unsigned)(cache->tokens - t0 < at_once ? cache->tokens - t0 : at_once);
+    for (long long t0 = 0; t0 < cache->tokens; t0 += plan.at_once) {
         p.t0 = (int)t0;
-        const dim3 grid((cache->table_width + SCORE_PAGES - 1) / SCORE_PAGES, cache->kv_heads, n);
-        cudaError_t e = cache->dtype == FCS_DTYPE_BF16 ? launch(score_kernel<true>, grid, SCORE_THREADS, 0, 1, stream, p)
-                                                       : launch(score_kernel<false>, grid, SCORE_THREADS, 0, 1, stream, p);
-        if (e == cudaSuccess) e = launch(choose_kernel, dim3(cache->kv_heads, n), CHOOSE_THREADS, 0, 1, stream, p);
+        p.t1 = (int)(cache->tokens - t0 < plan.at_once ? cache->tokens : t0 + plan.at_once);
+        const cudaError_t e = cache->dtype == FCS_DTYPE_BF16 ? launch_select<true>(p, plan.tiles, stream)
+                                                             : launch_select<false>(p, plan.tiles, stream);
         if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "choosing pages failed to launch: %s", cudaGetErrorString(e));
     }
     return FCS_OK;
@@ -311,7 +425,7 @@ int fcs_append_paged(const FcsPagedCache* cache, const FcsPagedRows* rows, int* 
 
 size_t fcs_select_pages_workspace_bytes(const FcsPagedCache* cache) {
     if (!cache || cache->tokens <= 0 || cache->kv_heads <= 0 || cache->table_width <= 0) return 0;
-    return fcs::paged::select_workspace(cache);
+    return fcs::paged::select_plan(cache).bytes;
 }
 
 int fcs_select_pages(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const void* bounds,

@@ -190,6 +190,13 @@ SELECTS = [
     ([70], [16 * 300], 16, 1, 8, 128, FP16, 40, 3, 4),
     ([1] * 270, [1 + 3 * i for i in range(270)], 16, 1, 2, 16, FP16, 5, 1, 1),
     ([2], [16 * 2100], 16, 1, 4, 32, BF16, 1500, 1, 1),
+    ([1], [16 * 2100 - 5], 16, 2, 4, 128, FP16, 33, 1, 2),
+    # many tokens a sequence: pages up to 512, up to 1024, more
+    ([70, 3, 0, 129], [16 * 300, 90, 7, 16 * 140 + 3], 16, 2, 6, 104, BF16, 21, 1, 1),
+    ([40], [16 * 1000], 16, 1, 2, 64, BF16, 64, 1, 1),
+    ([40], [16 * 900 + 7], 16, 1, 2, 128, FP16, 300, 0, 2),
+    ([24], [16 * 1500], 16, 1, 8, 96, BF16, 50, 1, 1),
+    ([24, 8], [16 * 1300, 16 * 1400], 16, 1, 1, 8, FP16, 700, 1, 1),
 ]
 
 
@@ -221,9 +228,10 @@ def test_select_takes_the_best_pages(case, ties):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-def test_select_orders_scores_that_differ_in_the_last_bits(dtype):
+@pytest.mark.parametrize("tokens,pages", [(4, 90), (20, 90), (9, 700), (9, 1100)])
+def test_select_orders_scores_that_differ_in_the_last_bits(dtype, tokens, pages):
     """Scores whose large terms cancel, so that sums in 32 bits could not tell the pages apart."""
-    a = Batch(3, [4], [16 * 90], 16, 2, 4, 64, dtype)
+    a = Batch(3, [tokens], [16 * pages], 16, 2, 4, 64, dtype)
     query = a.rows(4).abs() + 1
     bounds = torch.zeros(a.N, 2, 2, 64, dtype=dtype)
     bounds[:, :, 1] = torch.randn(a.N, 2, 64, generator=a.g).to(dtype)
@@ -235,8 +243,36 @@ def test_select_orders_scores_that_differ_in_the_last_bits(dtype):
     assert torch.equal(select(a, query, bounds, 11, 1, 1).cpu(), want)
 
 
-def test_select_with_infinities_nan_and_pages_that_the_table_lacks():
-    a = Batch(4, [3, 1], [16 * 60, 16 * 30], 16, 2, 2, 64, BF16)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens", [3, 16])
+def test_select_with_the_largest_values_of_the_type(dtype, tokens):
+    """Sums that overflow 32 bits (bf16) or parts that overflow 16 (fp16) are sums in 64 bits like any other."""
+    a = Batch(14, [tokens], [16 * 70], 16, 1, 8, 32, dtype)
+    most = torch.finfo(dtype).max
+    query = (torch.rand(a.T, 8, 32, generator=a.g) * most).to(dtype)
+    centre = torch.rand(a.N, 1, 32, generator=a.g) * 0.5
+    bounds = (torch.stack([centre, centre + 0.4], 2) * most).to(dtype)
+    want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, 9, 1, 1)
+    assert torch.equal(select(a, query, bounds, 9, 1, 1).cpu(), want)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    small_query, small_bounds = (query.double() / most * 64 * tiny).to(dtype), (bounds.double() / most * 64 * tiny).to(dtype)
+    want = chosen_pages(small_query, small_bounds, 16, a.table, a.lens, a.starts, 9, 1, 1)
+    assert torch.equal(select(a, small_query, small_bounds, 9, 1, 1).cpu(), want)
+
+
+def test_select_in_several_launches_under_a_wide_table():
+    """A table far wider than the sequences are long: the scores of all tokens at once would take a gigabyte."""
+    a = Batch(15, [70, 0, 30], [16 * 40, 5, 16 * 30], 16, 16, 16, 64, BF16, tail=5, width=60000)
+    query = a.rows(16)
+    bounds = torch.stack([a.normal(a.N, 16, 64) - 1, a.normal(a.N, 16, 64) + 1], 2)
+    want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, 6, 1, 1)
+    assert torch.equal(select(a, query, bounds, 6, 1, 1).cpu(), want)
+    status_is(0)
+
+
+@pytest.mark.parametrize("more", [0, 20])
+def test_select_with_infinities_nan_and_pages_that_the_table_lacks(more):
+    a = Batch(4, [3 + more, 1 + more], [16 * 60, 16 * 30], 16, 2, 2, 64, BF16)
     query = a.rows(2)
     bounds = torch.stack([a.normal(a.N, 2, 64) - 1, a.normal(a.N, 2, 64) + 1], 2)
     bounds[int(a.table[0, 20]), 0, 1, 3] = math.nan
