@@ -83,23 +83,18 @@ __device__ __forceinline__ unsigned long long key_of(double s) {
     return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
 }
 
-// E for a row whose parts sum up to `size` in magnitude, over pages whose bounds reach up to `reach`.  Sums that may overflow
-// are no sums (NaN likewise), and products that underflow lose what no share of the whole covers: 1e-36 is 85 times
-// the smallest normal number.
-__device__ __forceinline__ float error_of(float c, float size, float reach) {
-    const float most = size * reach;
-    return most < 1e37f ? c * most + 1e-36f : INFINITY;
-}
-
-// E of scores that matrix instructions formed of parts in two 16-bit pieces, 16 terms at a time.  Roundings of 2^-24: the group's
-// sums and the additions of D / 8 steps; in a step up to 2^-23 of each of 17 terms, where a tensor core drops what lies below the
-// last bit of the largest; what the pieces leave, 2^-18 (bf16) or 2^-22 (fp16) of a part, and half of fp16's smallest step of
-// every part.
+// E of a row whose parts sum up to `size` in magnitude and are at most `most`, over pages whose bounds reach up to `reach`; the
+// scores were formed by matrix instructions, 16 terms at a time from zero, of parts in `pieces` 16-bit pieces.  Of the whole's
+// magnitude: roundings of 2^-24, the group's sums and `adds` sums behind the matrix instructions, and what the pieces leave.  Of
+// the largest term: in each of D / 8 steps up to 2^-23 for 17 terms, where a tensor core drops what lies below its last bit.  And
+// half of fp16's smallest step of every part.  Sums that may overflow are no sums (NaN likewise), and products that underflow
+// lose what no share of the whole covers: 1e-36 is 85 times the smallest normal number.
 template <bool BF16>
-__device__ __forceinline__ float score_error(const SelectParams& p, float size, float reach) {
-    const float error = error_of((float)(p.group + p.c.dim / 8 + 36) * 6.5e-8f + (BF16 ? 3.9e-6f : 2.4e-7f), size, reach);
-    if constexpr (BF16) return error;
-    return size < 6e4f ? error + 2.f * p.c.dim * 3e-8f * reach : INFINITY;
+__device__ __forceinline__ float score_error(const SelectParams& p, float size, float most, float reach, int adds, int pieces) {
+    const float left = BF16 ? (pieces == 2 ? 3.9e-6f : 0.f) : (pieces == 2 ? 2.4e-7f : 0.f);
+    float error = ((float)(p.group + adds + 2) * 6.1e-8f + left) * size + (float)p.c.dim / 8.f * 17.f * 1.2e-7f * most;
+    if (!BF16) error = size < 6e4f ? error + 2.f * p.c.dim * 3e-8f : INFINITY;
+    return size * reach < 1e37f ? error * reach + 1e-36f : INFINITY;
 }
 
 // The largest magnitude among 16-bit values whose bit patterns, as unsigned and as signed integers, go up to these pairs: the
@@ -112,28 +107,56 @@ __device__ __forceinline__ float reach_of(uint32_t as_unsigned, uint32_t as_sign
     return max_or_nan(max_or_nan(x.x, x.y), max_or_nan(y.x, y.y));
 }
 
-// A page's score in 64 bits, by a warp.
+// A row's scores in 64 bits, by a warp: a lane has eight of the 2 D parts, the first D of which meet the lows.
 template <bool BF16>
-__device__ double exact_score(const SelectParams& p, const Row& r, int i) {
-    const Batch& c = p.c;
-    const int page = physical_page(c, r.b, i);
-    if (page < 0) return -INFINITY;
-    const uint16_t* at = p.bounds + ((long long)page * c.kv_heads + r.h) * 2 * c.dim;
-    double score = 0.0;
-    for (int d = threadIdx.x & 31; d < c.dim; d += 32) {
-        const uint16_t* q = p.query + r.t * p.query_st[0] + (long long)r.h * p.group * p.query_st[1] + d;
-        double n = 0.0, s = 0.0;
-        for (int g = 0; g < p.group; ++g, q += p.query_st[1]) {
-            const double x = widen16<BF16>(*q);
-            n += x < 0.0 ? x : 0.0;
-            s += x < 0.0 ? 0.0 : x;      // (NaN stays)
-        }
-        score += n * (double)widen16<BF16>(at[d]) + s * (double)widen16<BF16>(at[c.dim + d]);
-    }
+struct ExactScores {
+    double part[8];
+    __device__ ExactScores(const SelectParams& p, const Row& r) {
+        const int lane = threadIdx.x & 31, half = p.c.dim / 8;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) score += __shfl_xor_sync(0xffffffffu, score, o);
-    return score;
-}
+        for (int i = 0; i < 8; ++i) part[i] = 0.0;
+        if (lane >= 2 * half) return;
+        const bool low = lane < half;
+        const uint16_t* q = p.query + r.t * p.query_st[0] + (long long)r.h * p.group * p.query_st[1] + (low ? lane : lane - half) * 8;
+#pragma unroll 4
+        for (int g = 0; g < p.group; ++g) {
+            const uint4 w = *reinterpret_cast<const uint4*>(q + g * p.query_st[1]);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 x = widen_pair<BF16>(words[i]);
+                part[2 * i] += (low ? x.x < 0.f : !(x.x < 0.f)) ? (double)x.x : 0.0;      // (NaN stays)
+                part[2 * i + 1] += (low ? x.y < 0.f : !(x.y < 0.f)) ? (double)x.y : 0.0;
+            }
+        }
+    }
+    __device__ double operator()(const SelectParams& p, const Row& r, int i) const {
+        const Batch& c = p.c;
+        const int lane = threadIdx.x & 31, page = physical_page(c, r.b, i);
+        if (page < 0) return -INFINITY;
+        double score = 0.0;
+        if (lane < c.dim / 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p.bounds + ((long long)page * c.kv_heads + r.h) * 2 * c.dim + lane * 8);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 x = widen_pair<BF16>(words[e]);
+                score += part[2 * e] * (double)x.x;
+                score += part[2 * e + 1] * (double)x.y;
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) score += __shfl_xor_sync(0xffffffffu, score, o);
+        return score;
+    }
+};
+
+// Pages whose scores are too close to tell, up to 32 of them (shared memory of a team).
+struct CloseList {
+    unsigned long long key[32];
+    int page[32];
+    uint32_t n;
+};
 
 // ---- who chooses for a row: a block, or a warp.  A thread holds the keys of E consecutive pages (a block goes over more than
 // NT E pages in tiles, reading the scores again); key 0 is a page that does not compete.
@@ -152,11 +175,21 @@ __device__ __forceinline__ void load_keys(const Row& r, const float* scores, int
     }
 }
 
+__device__ __forceinline__ uint32_t warp_upto(uint32_t n) {       // inclusive sum over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, n, o);
+        if ((int)(threadIdx.x & 31) >= o) n += up;
+    }
+    return n;
+}
+
 template <int NT, int E>
 struct BlockTeam {
-    static constexpr int SIZE = NT, RUN = E, BINS = 512;
+    static constexpr int SIZE = NT, RUN = E, BINS = 4 * NT;
     const float* scores;
-    uint32_t* bins;              // shared: [BINS]
+    uint32_t* bins;              // shared: [BINS], zeros at first
+    CloseList* close;            // shared
     uint32_t* room;              // shared: [2][3 * NT / 32]
     int turn = 0;
     uint32_t keys[E];
@@ -204,13 +237,23 @@ struct BlockTeam {
         }
         return sum;
     }
-    __device__ static uint32_t warp_upto(uint32_t n) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(0xffffffffu, n, o);
-            if ((int)(threadIdx.x & 31) >= o) n += up;
+    // The bin that the `need`-th entry from the top is in, what is above it, and its count.
+    __device__ void locate(uint32_t need, uint32_t& above, uint32_t& bin, uint32_t& count) {
+        const uint32_t at = BINS - 4 * (threadIdx.x + 1);
+        const uint4 q = *reinterpret_cast<const uint4*>(&bins[at]);
+        uint32_t total;
+        const uint32_t from = before(q.x + q.y + q.z + q.w, total);
+        if (from < need && need <= from + q.x + q.y + q.z + q.w) {
+            const uint32_t a3 = from + q.w, a2 = a3 + q.z, a1 = a2 + q.y;
+            const int i = need <= a3 ? 3 : need <= a2 ? 2 : need <= a1 ? 1 : 0;
+            close->n = at + i;                 // (free until a list is made)
+            close->page[0] = (int)(i == 3 ? from : i == 2 ? a3 : i == 1 ? a2 : a1);
+            close->page[1] = (int)(i == 3 ? q.w : i == 2 ? q.z : i == 1 ? q.y : q.x);
         }
-        return n;
+        __syncthreads();
+        bin = close->n;
+        above = (uint32_t)close->page[0];
+        count = (uint32_t)close->page[1];
     }
 };
 
@@ -218,7 +261,8 @@ template <int E>
 struct WarpTeam {
     static constexpr int SIZE = 32, RUN = E, BINS = 256;
     const float* scores;
-    uint32_t* bins;              // shared: [BINS], the warp's own
+    uint32_t* bins;              // shared, the warp's own: [BINS], zeros at first
+    CloseList* close;            // shared, the warp's own
     uint32_t keys[E];
     __device__ int rank() const { return threadIdx.x & 31; }
     __device__ void sync() const { __syncwarp(); }
@@ -233,9 +277,37 @@ struct WarpTeam {
         for (int j = 0; j < 3; ++j) v[j] = op.warp(v[j]);
     }
     __device__ uint32_t before(uint32_t n, uint32_t& total) const {
-        const uint32_t upto = BlockTeam<32, 1>::warp_upto(n);
+        const uint32_t upto = warp_upto(n);
         total = __shfl_sync(0xffffffffu, upto, 31);
         return upto - n;
+    }
+    __device__ void locate(uint32_t need, uint32_t& above, uint32_t& bin, uint32_t& count) const {
+        constexpr int PER = BINS / 32;
+        const int lane = rank();
+        uint32_t n[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>(&bins[BINS - PER * (lane + 1) + i]);
+            n[i] = q.x, n[i + 1] = q.y, n[i + 2] = q.z, n[i + 3] = q.w;
+            sum += q.x + q.y + q.z + q.w;
+        }
+        const uint32_t upto = warp_upto(sum);
+        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
+        above = upto - sum;
+        bin = count = 0;
+        bool open = true;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) {
+            if (open && above + n[i] >= need) {
+                open = false;
+                bin = BINS - PER * (lane + 1) + i;
+                count = n[i];
+            }
+            if (open) above += n[i];
+        }
+        above = __shfl_sync(0xffffffffu, above, owner);
+        bin = __shfl_sync(0xffffffffu, bin, owner);
+        count = __shfl_sync(0xffffffffu, count, owner);
     }
 };
 
@@ -252,52 +324,26 @@ struct Largest {
 // than `need` of them.  A histogram over the range, and again over the bin that holds the place, until a bin is wanted whole.
 template <typename Team>
 __device__ uint32_t kth_key(const Row& r, Team& team, uint32_t need, uint32_t low, uint32_t high, bool& clean) {
-    constexpr int BINS = Team::BINS, PER = BINS / 32;
-    const int lane = threadIdx.x & 31;
+    constexpr int BINS = Team::BINS;
     while (true) {
         const int width = 32 - __clz(high - low);      // bits of the range
         const int shift = max(0, width - (31 - __clz(BINS)));
-        team.sync();                                   // (the bins of the round before have been read)
-        for (int i = team.rank(); i < BINS; i += Team::SIZE) team.bins[i] = 0;
-        team.sync();
         team.tiles(r, [&](int) {
 #pragma unroll
             for (int j = 0; j < Team::RUN; ++j)
-                if (team.keys[j] >= low && team.keys[j] <= high && team.keys[j])
-                    atomicAdd(&team.bins[(team.keys[j] - low) >> shift], 1u);
+                if (team.keys[j] >= low && team.keys[j] <= high) atomicAdd(&team.bins[(team.keys[j] - low) >> shift], 1u);
         });
         team.sync();
-        // every warp for itself: lane i has the i-th run of bins from the top
-        uint32_t n[PER], sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(&team.bins[BINS - PER * (lane + 1) + i]);
-            n[i] = q.x, n[i + 1] = q.y, n[i + 2] = q.z, n[i + 3] = q.w;
-            sum += q.x + q.y + q.z + q.w;
-        }
-        const uint32_t upto = BlockTeam<32, 1>::warp_upto(sum);
-        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
-        uint32_t above = upto - sum, bin = 0, count = 0;
-        if (lane == owner) {
-            bool open = true;
-#pragma unroll
-            for (int i = PER - 1; i >= 0; --i) {
-                if (open && above + n[i] >= need) {
-                    open = false;
-                    bin = BINS - PER * (lane + 1) + i;
-                    count = n[i];
-                }
-                if (open) above += n[i];
-            }
-        }
-        above = __shfl_sync(0xffffffffu, above, owner);
-        bin = __shfl_sync(0xffffffffu, bin, owner);
-        count = __shfl_sync(0xffffffffu, count, owner);
+        uint32_t above, bin, count;
+        team.locate(need, above, bin, count);
         need -= above;
         low += bin << shift;
         clean = count == need;
         if (clean || shift == 0) return low;
         high = low + ((1u << shift) - 1);
+        team.sync();                                   // (all have read the bins)
+        for (int i = team.rank() * 4; i < BINS; i += Team::SIZE * 4) *reinterpret_cast<uint4*>(&team.bins[i]) = make_uint4(0, 0, 0, 0);
+        team.sync();
     }
 }
 
@@ -328,26 +374,28 @@ __device__ unsigned long long kth_wide_key(Team& team, uint32_t need, unsigned l
     return low;
 }
 
-// Chooses the pages of a row and writes them.  `error`: E.  `exact`: the row's memory for sums in 64 bits.
+// Chooses the pages of a row and writes them.  `ends`: the largest key and the complement of the smallest, or zeros.  `error`: E.
+// `exact`: the row's memory for sums in 64 bits.
 template <bool BF16, typename Team>
-__device__ void choose(const SelectParams& p, const Row& r, Team& team, float error, double* exact, int* out) {
+__device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t (&ends)[3], float error, double* exact, int* out) {
     constexpr int E = Team::RUN;
     uint32_t(&keys)[E] = team.keys;
     team.load(r, 0);
     // keys above `sure` are chosen, keys from `open` on may be
     uint32_t sure = 0xffffffffu, open = 0xffffffffu;
     unsigned long long bar = ~0ull;       // of the latter: 64-bit keys above `bar`, and the first `equal` at it
-    uint32_t equal = 0;
+    uint32_t equal = 0, picked = 0;       // or of a list of them, the picked
     if (r.need > 0) {
-        uint32_t ends[3] = {0, 0, 0};     // the largest key, the complement of the smallest
-        team.tiles(r, [&](int) {
+        if (ends[0] == 0) {
+            team.tiles(r, [&](int) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                ends[0] = max(ends[0], keys[j]);
-                if (keys[j]) ends[1] = max(ends[1], ~keys[j]);
-            }
-        });
-        team.reduce(ends, Largest());
+                for (int j = 0; j < E; ++j) {
+                    ends[0] = max(ends[0], keys[j]);
+                    if (keys[j]) ends[1] = max(ends[1], ~keys[j]);
+                }
+            });
+            team.reduce(ends, Largest());
+        }
         bool clean;
         uint32_t kth = kth_key(r, team, r.need, ~ends[1], ends[0], clean);
         bool apart = false;
@@ -382,9 +430,13 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, float er
             });
             team.reduce(n, Sum());
             const uint32_t left = r.need - n[0];
+            const bool listed = n[1] <= 32;
             if (n[1] == left) {           // all of them
                 bar = 0;
             } else {
+                if (team.rank() == 0) team.close->n = 0;
+                team.sync();
+                const ExactScores<BF16> score(p, r);
                 team.tiles(r, [&](int i) {
 #pragma unroll
                     for (int j = 0; j < E; ++j) {
@@ -393,12 +445,32 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, float er
                             const int src = __ffs(todo) - 1;
                             todo &= todo - 1;
                             const int page = __shfl_sync(0xffffffffu, i, src) + j;
-                            const double s = exact_score<BF16>(p, r, page);
-                            if ((int)(threadIdx.x & 31) == src) exact[page] = s;
+                            const double s = score(p, r, page);
+                            if ((int)(threadIdx.x & 31) == src) {
+                                if (listed) {
+                                    const uint32_t at = atomicAdd(&team.close->n, 1u);
+                                    team.close->key[at] = key_of(s);
+                                    team.close->page[at] = page;
+                                } else {
+                                    exact[page] = s;
+                                }
+                            }
                         }
                     }
                 });
                 team.sync();
+            }
+            if (n[1] != left && listed) {       // every warp for itself: how many are before a lane's page
+                const int lane = threadIdx.x & 31, m = (int)n[1];
+                const unsigned long long key = lane < m ? team.close->key[lane] : 0ull;
+                const int page = lane < m ? team.close->page[lane] : 0;
+                uint32_t ahead = 0;
+                for (int i = 0; i < m; ++i) {
+                    const unsigned long long other = team.close->key[i];
+                    ahead += other > key || (other == key && team.close->page[i] < page);
+                }
+                picked = __ballot_sync(0xffffffffu, lane < m && ahead < left);
+            } else if (n[1] != left) {
                 auto over_open = [&](auto count) {
                     team.tiles(r, [&](int i) {
 #pragma unroll
@@ -427,9 +499,13 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, float er
         for (int j = 0; j < E; ++j) {
             bool take = i + j < r.pages && (keys[j] == 0 || keys[j] > sure);
             if (keys[j] >= open && keys[j] <= sure) {
-                const unsigned long long wide = bar == 0 ? 1ull : key_of(exact[i + j]);
-                take = wide > bar;
-                if (wide == bar) same |= 1u << j;
+                if (picked) {
+                    for (uint32_t left = picked; left; left &= left - 1) take |= team.close->page[__ffs(left) - 1] == i + j;
+                } else {
+                    const unsigned long long wide = bar == 0 ? 1ull : key_of(exact[i + j]);
+                    take = wide > bar;
+                    if (wide == bar) same |= 1u << j;
+                }
             }
             if (take) taken |= 1u << j;
         }
@@ -469,11 +545,14 @@ template <bool BF16, int DP, int CL>
 __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid_constant__ SelectParams p) {
     constexpr int CHUNKS = DP / 16;               // 32 of the 2 D features
     extern __shared__ __align__(16) float row_scores[];
-    __shared__ float reach_of_cta[CL];
-    __shared__ float warp_reach[ROW_THREADS / 32], warp_size[ROW_THREADS / 32];
-    __shared__ uint32_t room[2 * 3 * ROW_THREADS / 32];
+    constexpr int WARPS = ROW_THREADS / 32;
+    __shared__ uint32_t of_cta[3][CL];            // the largest key, the complement of the smallest, the reach
+    __shared__ uint32_t of_warp[3][WARPS];
+    __shared__ float warp_size[WARPS], warp_most[WARPS];
+    __shared__ uint32_t room[2 * 3 * WARPS];
+    __shared__ CloseList close;
     __shared__ __align__(16) uint32_t bins[RowTeam::BINS];
-    __shared__ __align__(16) uint16_t parts[3][2 * DP];       // what 16 bits hold, the rest, zeros
+    __shared__ __align__(16) uint16_t parts[4][2 * DP];       // what 16 bits hold, the rest of that and the rest's, zeros
     if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     grid_dependency_wait();
     grid_launch_dependents();
@@ -495,17 +574,22 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
                 part += (low ? x < 0.f : !(x < 0.f)) ? x : 0.f;      // (NaN stays)
             }
         }
-        float rest, z;
+        float rest, rest2, z;
         parts[0][tid] = (uint16_t)round_pair<BF16>(part, 0.f, rest, z);
-        parts[1][tid] = (uint16_t)round_pair<BF16>(rest, 0.f, z, z);
-        parts[2][tid] = 0;
-        float size = fabsf(part);
+        parts[1][tid] = (uint16_t)round_pair<BF16>(rest, 0.f, rest2, z);
+        parts[2][tid] = (uint16_t)round_pair<BF16>(rest2, 0.f, z, z);
+        parts[3][tid] = 0;
+        float size = fabsf(part), most = size;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) size += __shfl_xor_sync(0xffffffffu, size, o);
-        if (lane == 0) warp_size[warp] = size;
+        for (int o = 16; o > 0; o >>= 1) {
+            size += __shfl_xor_sync(0xffffffffu, size, o);
+            most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        if (lane == 0) warp_size[warp] = size, warp_most[warp] = most;
     } else if (lane == 0) {
-        warp_size[warp] = 0.f;
+        warp_size[warp] = warp_most[warp] = 0.f;
     }
+    *reinterpret_cast<uint4*>(&bins[tid * 4]) = make_uint4(0, 0, 0, 0);
     Row r = {};
     if (b < c.sequences) r.set(p, t, h, b, pos);
     int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
@@ -525,7 +609,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     uint32_t to = smem_u32(row_scores);
     if constexpr (CL > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(to), "r"(0));
     const int row = lane >> 2, col = lane & 3;
-    const uint16_t* columns = parts[min(row, 2)] + col * 8;
+    const uint16_t* columns = parts[min(row, 3)] + col * 8;
+    uint32_t ends[3] = {0, 0, 0};
     while (base < end) {
         const int page0 = __shfl_sync(0xffffffffu, entry, row), page1 = __shfl_sync(0xffffffffu, entry, row + 8);
         const bool there0 = page0 >= 0 && page0 < c.pages, there1 = page1 >= 0 && page1 < c.pages;
@@ -546,7 +631,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const uint4 f = *reinterpret_cast<const uint4*>(columns + (s0 + s) * 32);
-                // (every step starts from zero: see score_error)
+                // (every instruction starts from zero: see score_error)
                 float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
                 const uint32_t a0[4] = {w0[s].x, w1[s].x, w0[s].y, w1[s].y}, a1[4] = {w0[s].z, w1[s].z, w0[s].w, w1[s].w};
                 mma16816<BF16>(x, a0, f.x, f.y);
@@ -563,14 +648,18 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
                 low_bits = __vimax3_s16x2(low_bits, w1[s].z, w1[s].w);
             }
         }
-        if (col < 2) {          // column 0 and 1 together are the score; lane 4 i has page i's and page i + 8's
+        // columns 0 to 2 together are the score; lane 4 i has 0 and 1 of pages i and i + 8, lane 4 i + 1 has 2
+        const float third0 = __shfl_down_sync(0xffffffffu, acc[0], 1), third1 = __shfl_down_sync(0xffffffffu, acc[2], 1);
+        const float second = __shfl_up_sync(0xffffffffu, (acc[2] + acc[3]) + third1, 1);
+        if (col < 2) {
             const int i = base + row + 8 * col;
-            const float other = __shfl_sync(0x33333333u, acc[2] + acc[3], lane & ~1);
-            const float score = col == 0 ? acc[0] + acc[1] : other;
             const bool there = col == 0 ? there0 : there1;
             if (i < end) {
                 lacking |= !there;
-                const float s = there ? score : -INFINITY;
+                const float s = !there ? -INFINITY : col == 0 ? (acc[0] + acc[1]) + third0 : second;
+                const uint32_t key = key_of(s);
+                ends[0] = max(ends[0], key);
+                ends[1] = max(ends[1], ~key);
                 if constexpr (CL > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(s) : "memory");
                 else row_scores[i] = s;
             }
@@ -579,34 +668,48 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
         base = next;
     }
     if (lacking) report(c, FCS_STATUS_BAD_PAGE);
-    float most = reach_of<BF16>(high_bits, low_bits);
+    // (the reach is not negative, or NaN: its bits are in order)
+    ends[2] = __float_as_uint(reach_of<BF16>(high_bits, low_bits));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) warp_reach[warp] = most;
+    for (int i = 0; i < 3; ++i) {
+        ends[i] = __reduce_max_sync(0xffffffffu, ends[i]);
+        if (lane == 0) of_warp[i][warp] = ends[i];
+    }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < ROW_THREADS / 32; ++w) most = max_or_nan(most, warp_reach[w]);
-        if constexpr (CL > 1) {
-            uint32_t at;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&reach_of_cta[rank])), "r"(0));
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(most) : "memory");
-        } else {
-            reach_of_cta[0] = most;
+    if (warp == 0) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ends[i] = __reduce_max_sync(0xffffffffu, lane < WARPS ? of_warp[i][lane] : 0u);
+        if (lane < 3) {
+            const uint32_t mine = lane == 0 ? ends[0] : lane == 1 ? ends[1] : ends[2];
+            uint32_t at = smem_u32(&of_cta[lane][rank]);
+            if constexpr (CL > 1) {
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(at), "r"(0));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(mine) : "memory");
+            } else {
+                of_cta[lane][rank] = mine;
+            }
         }
+        __syncwarp();
     }
     if constexpr (CL > 1) {
-        __syncwarp();
         cluster_sync();
         if (rank > 0) return;
     } else {
         __syncthreads();
     }
-    most = reach_of_cta[0];
-    for (int i = 1; i < CL; ++i) most = max_or_nan(most, reach_of_cta[i]);
-    float size = 0.f;
-    for (int w = 0; w < ROW_THREADS / 32; ++w) size += warp_size[w];
-    RowTeam team{row_scores, bins, room};
-    choose<BF16>(p, r, team, score_error<BF16>(p, size, most), p.exact + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch, out);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) ends[i] = __reduce_max_sync(0xffffffffu, lane < CL ? of_cta[i][lane] : 0u);
+    float size = lane < WARPS ? warp_size[lane] : 0.f, most = lane < WARPS ? warp_most[lane] : 0.f;
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+        size += __shfl_xor_sync(0xffffffffu, size, o);
+        most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    size = __shfl_sync(0xffffffffu, size, 0);
+    most = __shfl_sync(0xffffffffu, most, 0);
+    RowTeam team{row_scores, bins, &close, room};
+    const float error = score_error<BF16>(p, size, most, __uint_as_float(ends[2]), CHUNKS + 3, 3);
+    choose<BF16>(p, r, team, ends, error, p.exact + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch, out);
 }
 
 // ------------------------------------------------------------------ many tokens a sequence
@@ -622,7 +725,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid_constant__ SelectParams p) {
     extern __shared__ __align__(16) uint8_t tiles_smem_raw[];
     __shared__ uint32_t reach_of_warp[TILES_THREADS / 32];
-    __shared__ float size_of_token[TILE_TOKENS];
+    __shared__ float size_of_token[TILE_TOKENS], most_of_token[TILE_TOKENS];
     __shared__ uint8_t missing[TILE_PAGES];
     grid_dependency_wait();
     grid_launch_dependents();
@@ -652,7 +755,7 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
     uint8_t* const tile = lo + TILE_TOKENS * row_bytes;  // [pages][2 D]
     const int my_row = tid >> 2, my_vec = tid & 3;       // four threads a row
     {
-        float size = 0.f;
+        float size = 0.f, most = 0.f;
         for (int v = my_vec; v < D / 8; v += 4) {
             float n[8], s[8];
 #pragma unroll
@@ -673,7 +776,10 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) size += s[i] - n[i];
+            for (int i = 0; i < 8; ++i) {
+                size += s[i] - n[i];
+                most = max_or_nan(most, max_or_nan(s[i], -n[i]));
+            }
             uint32_t nh[4], nl[4], sh[4], sl[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -691,7 +797,9 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
         }
         size += __shfl_xor_sync(0xffffffffu, size, 1);
         size += __shfl_xor_sync(0xffffffffu, size, 2);
-        if (my_vec == 0) size_of_token[my_row] = size;
+        most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if (my_vec == 0) size_of_token[my_row] = size, most_of_token[my_row] = most;
     }
 
     const int wm = warp & 3, wn = warp >> 2;
@@ -765,7 +873,7 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
     if (tid < tokens && t_first + tid >= p.t0 && t_first + tid < p.t1) {
         for (int w = 0; w < TILES_THREADS / 32; ++w) most = max_or_nan(most, __uint_as_float(reach_of_warp[w]));
         p.errors[((long long)(t_first + tid - p.t0) * c.kv_heads + h) * p.splits + blockIdx.z] =
-            score_error<BF16>(p, size_of_token[tid], most);
+            score_error<BF16>(p, size_of_token[tid], most_of_token[tid], most, D / 8, 2);
     }
 }
 
@@ -779,6 +887,9 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_con
     typedef WarpTeam<(E > 0 ? E : 4)> Warp;
     __shared__ uint32_t room[2 * 3 * CHOOSE_THREADS / 32];
     __shared__ __align__(16) uint32_t bins[E > 0 ? ROWS * Warp::BINS : Block::BINS];
+    __shared__ CloseList close[ROWS];
+    for (int i = threadIdx.x; i < (int)(sizeof(bins) / 4); i += CHOOSE_THREADS) bins[i] = 0;
+    __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
     const Batch& c = p.c;
@@ -803,12 +914,13 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_con
     float error = 0.f;
     for (int s = 0; s < p.splits; ++s) error = max_or_nan(error, p.errors[row * p.splits + s]);
     if (!(error < INFINITY)) error = INFINITY;
+    uint32_t ends[3] = {0, 0, 0};
     if constexpr (E > 0) {
-        Warp team{scores, bins + (threadIdx.x >> 5) * Warp::BINS};
-        choose<BF16>(p, r, team, error, exact, out);
+        Warp team{scores, bins + (threadIdx.x >> 5) * Warp::BINS, &close[threadIdx.x >> 5]};
+        choose<BF16>(p, r, team, ends, error, exact, out);
     } else {
-        Block team{scores, bins, room};
-        choose<BF16>(p, r, team, error, exact, out);
+        Block team{scores, bins, close, room};
+        choose<BF16>(p, r, team, ends, error, exact, out);
     }
 }
 
