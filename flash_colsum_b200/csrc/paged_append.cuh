@@ -20,7 +20,7 @@
 namespace fcs {
 namespace paged {
 
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_THREADS = 128;
 
 struct AppendParams {
     Batch c;
@@ -31,8 +31,10 @@ struct AppendParams {
     const float *cos, *sin;        // (table_rows, rotary / 2)
     const int* positions;          // or nullptr: where the token lies in its sequence
     int q_heads, rotary, interleaved, table_rows;
-    int heads_shift;               // heads of a CTA, as a power of two (at most 16)
-    int kv_groups;                 // CTAs over the key (and as many over the value) heads
+    int heads_shift;               // heads that a CTA has at a time, as a power of two (at most 16)
+    int steps;                     // and how often, of values and queries
+    int key_groups, value_groups;  // CTAs over the key heads, over the value heads
+    int groups;                    // and over all; the CTAs of a page are neighbours, so that rows are read and written whole
     int fill_tail;
 };
 
@@ -82,66 +84,76 @@ __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
     x = a;
 }
 
-// Eight pairs whose halves lie in two vectors.
-template <typename Ops>
-__device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float* cos, const float* sin) {
-    uint32_t* wa = reinterpret_cast<uint32_t*>(&a);
-    uint32_t* wb = reinterpret_cast<uint32_t*>(&b);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const float4 c = reinterpret_cast<const float4*>(cos)[h], s = reinterpret_cast<const float4*>(sin)[h];
-        float2 x0 = Ops::widen(wa[2 * h]), x1 = Ops::widen(wa[2 * h + 1]);
-        float2 y0 = Ops::widen(wb[2 * h]), y1 = Ops::widen(wb[2 * h + 1]);
-        turn(x0.x, y0.x, c.x, s.x);
-        turn(x0.y, y0.y, c.y, s.y);
-        turn(x1.x, y1.x, c.z, s.z);
-        turn(x1.y, y1.y, c.w, s.w);
-        wa[2 * h] = Ops::narrow(x0.x, x0.y);
-        wa[2 * h + 1] = Ops::narrow(x1.x, x1.y);
-        wb[2 * h] = Ops::narrow(y0.x, y0.y);
-        wb[2 * h + 1] = Ops::narrow(y1.x, y1.y);
+// The rotation of one token, for eight pairs whose halves lie in two vectors or four pairs side by side in one.
+struct Turn {
+    float4 c[2], s[2];
+    __device__ void load(const float* cos, const float* sin, bool both) {
+        c[0] = *reinterpret_cast<const float4*>(cos);
+        s[0] = *reinterpret_cast<const float4*>(sin);
+        if (both) {
+            c[1] = *reinterpret_cast<const float4*>(cos + 4);
+            s[1] = *reinterpret_cast<const float4*>(sin + 4);
+        }
     }
-}
-// Four pairs side by side in one vector.
-template <typename Ops>
-__device__ __forceinline__ void turn_neighbours(uint4& a, const float* cos, const float* sin) {
-    uint32_t* w = reinterpret_cast<uint32_t*>(&a);
-    const float4 c4 = *reinterpret_cast<const float4*>(cos), s4 = *reinterpret_cast<const float4*>(sin);
-    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+    template <typename Ops>
+    __device__ void halves(uint4& a, uint4& b) const {
+        uint32_t* wa = reinterpret_cast<uint32_t*>(&a);
+        uint32_t* wb = reinterpret_cast<uint32_t*>(&b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float2 v = Ops::widen(w[i]);
-        turn(v.x, v.y, c[i], s[i]);
-        w[i] = Ops::narrow(v.x, v.y);
+        for (int h = 0; h < 2; ++h) {
+            float2 x0 = Ops::widen(wa[2 * h]), x1 = Ops::widen(wa[2 * h + 1]);
+            float2 y0 = Ops::widen(wb[2 * h]), y1 = Ops::widen(wb[2 * h + 1]);
+            turn(x0.x, y0.x, c[h].x, s[h].x);
+            turn(x0.y, y0.y, c[h].y, s[h].y);
+            turn(x1.x, y1.x, c[h].z, s[h].z);
+            turn(x1.y, y1.y, c[h].w, s[h].w);
+            wa[2 * h] = Ops::narrow(x0.x, x0.y);
+            wa[2 * h + 1] = Ops::narrow(x1.x, x1.y);
+            wb[2 * h] = Ops::narrow(y0.x, y0.y);
+            wb[2 * h + 1] = Ops::narrow(y1.x, y1.y);
+        }
     }
-}
+    template <typename Ops>
+    __device__ void neighbours(uint4& a) const {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&a);
+        const float cc[4] = {c[0].x, c[0].y, c[0].z, c[0].w}, ss[4] = {s[0].x, s[0].y, s[0].z, s[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float2 v = Ops::widen(w[i]);
+            turn(v.x, v.y, cc[i], ss[i]);
+            w[i] = Ops::narrow(v.x, v.y);
+        }
+    }
+};
 
-template <typename Ops>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ AppendParams p) {
+// ROT: 0 nothing is rotated, 1 pairs are half the rotated part apart, 2 side by side
+template <typename Ops, int ROT>
+__global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ uint4 sums[APPEND_THREADS][4];
     grid_dependency_wait();
     grid_launch_dependents();
     const Batch& c = p.c;
-    const int P = 1 << c.page_shift, D = c.dim, heads_of_cta = 1 << p.heads_shift;
-    const int kind = (int)blockIdx.y < p.kv_groups ? 0 : (int)blockIdx.y < 2 * p.kv_groups ? 1 : 2;   // keys, values, queries
-    const int h0 = ((int)blockIdx.y - kind * p.kv_groups) << p.heads_shift;
-    const int heads = min(heads_of_cta, (kind == 2 ? p.q_heads : c.kv_heads) - h0);
+    const int D = c.dim, y = (int)(blockIdx.x % (unsigned)p.groups), segment = (int)(blockIdx.x / (unsigned)p.groups);
+    const int kind = y < p.key_groups ? 0 : y < p.key_groups + p.value_groups ? 1 : 2;   // keys, values, queries
+    const int steps = kind == 0 ? 1 : p.steps;
+    const int h0 = (y - (kind == 0 ? 0 : kind == 1 ? p.key_groups : p.key_groups + p.value_groups)) * (steps << p.heads_shift);
+    const int heads = min(steps << p.heads_shift, (kind == 2 ? p.q_heads : c.kv_heads) - h0);
 
     // the page of this CTA: sequence b, the j-th page that it writes
-    int b = (int)blockIdx.x;
+    int b = segment;
     long long j = 0, s0 = b, n = 1;
     if (c.starts) {
         int seen = 0;
         for (int base = 0; base < c.sequences; base += APPEND_THREADS) {
             const int i = base + (int)threadIdx.x + 1;
-            seen += __syncthreads_count(i <= c.sequences && (c.starts[i] >> c.page_shift) + 2ll * i <= blockIdx.x);
+            seen += __syncthreads_count(i <= c.sequences && (c.starts[i] >> c.page_shift) + 2ll * i <= segment);
         }
         b = seen;
         s0 = c.starts[b];
-        j = (long long)blockIdx.x - ((s0 >> c.page_shift) + 2ll * b);
+        j = (long long)segment - ((s0 >> c.page_shift) + 2ll * b);
         if (b == c.sequences) {     // no sequence: rows behind the last one
             if (kind != 2 || !p.fill_tail) return;
-            const long long step = (long long)gridDim.x - blockIdx.x + j;
+            const long long step = (long long)(gridDim.x / (unsigned)p.groups) - segment + j;
             for (long long t = max(s0, 0ll) + j; t < c.tokens; t += step)
                 for (int i = threadIdx.x; i < heads * (D / 8); i += APPEND_THREADS)
                     *reinterpret_cast<uint4*>(p.query_out + t * p.query_out_st[0] + (h0 + i / (D / 8)) * p.query_out_st[1] +
@@ -155,38 +167,89 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
     const long long page_index = (p0 >> c.page_shift) + j;
     const long long first = max(p0, page_index << c.page_shift), end = min(len, (page_index + 1) << c.page_shift);
     if (first >= end) return;
-    const int tokens = (int)(end - first), slot0 = (int)(first & (P - 1));
+    const int tokens = (int)(end - first), slot0 = (int)(first & ((1 << c.page_shift) - 1));
     const long long t0 = s0 + (first - p0);
     const int page = kind == 2 ? 0 : physical_page(c, b, page_index);
     if (page < 0) return;
 
-    const uint16_t* src = kind == 0 ? p.key : kind == 1 ? p.value : p.query;
-    const long long* src_st = kind == 0 ? p.key_st : kind == 1 ? p.value_st : p.query_st;
-    uint16_t* dst;
-    long long dst_head, dst_token;
-    if (kind == 2) {
-        dst = p.query_out + t0 * p.query_out_st[0];
-        dst_token = p.query_out_st[0];
-        dst_head = p.query_out_st[1];
-    } else {
-        const long long* st = kind == 0 ? p.key_page_st : p.value_page_st;
-        dst = (kind == 0 ? p.key_pages : p.value_pages) + page * st[0] + slot0 * st[2];
-        dst_token = st[2];
-        dst_head = st[1];
-    }
-
     // A thread keeps its features and its head: a vector of eight features, or two whose features are pairs.
-    const int R = kind == 1 ? 0 : p.rotary;
-    const bool halves = R > 0 && !p.interleaved;
-    const int pair_units = halves ? R / 16 : 0;
+    const int rotary = kind == 1 ? 0 : p.rotary;
+    const int pair_units = ROT == 1 ? rotary / 16 : 0;
     const int units = pair_units + (D - 16 * pair_units) / 8;
     const int rows = (APPEND_THREADS / units) >> p.heads_shift << p.heads_shift;    // (token, head) pairs at a time
     const int u = (int)threadIdx.x % units, r0 = (int)threadIdx.x / units;
-    const int head = r0 & (heads_of_cta - 1), lane = r0 >> p.heads_shift, lanes = rows >> p.heads_shift;
-    const bool paired = u < pair_units;
-    const int va = paired ? u : u + pair_units, vb = u + pair_units;          // vectors of the row
+    const int head = r0 & ((1 << p.heads_shift) - 1), lane = r0 >> p.heads_shift, lanes = rows >> p.heads_shift;
+    const bool paired = ROT == 1 && u < pair_units;
+    const int va = paired ? u : u + pair_units, apart = paired ? pair_units * 8 : 0;      // the vector, and how far the other is
+    const bool side_by_side = ROT == 2 && va * 8 < rotary;
     const bool mine = r0 < rows && head < heads;
-    const bool side_by_side = R > 0 && p.interleaved && va * 8 < R;
+
+    const long long src_token = kind == 0 ? p.key_st[0] : kind == 1 ? p.value_st[0] : p.query_st[0];
+    const long long src_head = kind == 0 ? p.key_st[1] : kind == 1 ? p.value_st[1] : p.query_st[1];
+    const long long dst_token = kind == 0 ? p.key_page_st[2] : kind == 1 ? p.value_page_st[2] : p.query_out_st[0];
+    const long long dst_head = kind == 0 ? p.key_page_st[1] : kind == 1 ? p.value_page_st[1] : p.query_out_st[1];
+    const uint16_t* src = (kind == 0 ? p.key : kind == 1 ? p.value : p.query) + (t0 + lane) * src_token + (h0 + head) * src_head + va * 8;
+    uint16_t* dst = kind == 2 ? p.query_out + t0 * dst_token
+                              : (kind == 0 ? p.key_pages + page * p.key_page_st[0] : p.value_pages + page * p.value_page_st[0]) + slot0 * dst_token;
+    dst += lane * dst_token + (h0 + head) * dst_head + va * 8;
+
+    // The rotation of a token is asked for; whether there is one.
+    auto turn_of = [&](int tok, Turn& turn) {
+        if (ROT == 0) return true;
+        const long long pos = p.positions ? (long long)p.positions[t0 + tok] : first + tok;
+        if (pos < 0 || pos >= p.table_rows) {
+            report(c, FCS_STATUS_BAD_POSITION);
+            return false;
+        }
+        const long long at = pos * (p.rotary / 2) + (ROT == 1 ? va * 8 : va * 4);
+        if (paired || side_by_side) turn.load(p.cos + at, p.sin + at, ROT == 1);
+        return true;
+    };
+    auto apply = [&](const Turn& turn, uint4& a, uint4& bb) {
+        if (paired) turn.halves<Ops>(a, bb);
+        if (side_by_side) turn.neighbours<Ops>(a);
+    };
+
+    if (kind != 0) {
+        // values and queries: a token's rotation serves its heads, which are asked for in twos
+        const long long src_step = src_head << p.heads_shift, dst_step = dst_head << p.heads_shift;
+        const int mine_steps = (heads - head + (1 << p.heads_shift) - 1) >> p.heads_shift;
+        for (int tok = mine ? lane : tokens; tok < tokens; tok += lanes) {
+            const uint16_t* from = src;
+            uint16_t* to = dst;
+            uint4 a0, b0, a1, b1;
+            auto ask = [&](int s, uint4& a, uint4& bb) {
+                if (s >= mine_steps) return;
+                a = *reinterpret_cast<const uint4*>(from);
+                if (paired) bb = *reinterpret_cast<const uint4*>(from + apart);
+                from += src_step;
+            };
+            ask(0, a0, b0);
+            ask(1, a1, b1);
+            Turn turn;
+            const bool good = turn_of(tok, turn);
+            auto write = [&](uint4& a, uint4& bb) {
+                if (good) apply(turn, a, bb);
+                else a = bb = make_uint4(0, 0, 0, 0);
+                if (good || kind == 2) {
+                    *reinterpret_cast<uint4*>(to) = a;
+                    if (paired) *reinterpret_cast<uint4*>(to + apart) = bb;
+                }
+                to += dst_step;
+            };
+            for (int s = 0; s < mine_steps; s += 2) {
+                if (s > 0) {
+                    ask(s, a0, b0);
+                    ask(s + 1, a1, b1);
+                }
+                write(a0, b0);
+                if (s + 1 < mine_steps) write(a1, b1);
+            }
+            src += lanes * src_token;
+            dst += lanes * dst_token;
+        }
+        return;
+    }
 
     uint4 low[2], high[2];
 #pragma unroll
@@ -194,37 +257,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
         low[i] = make_uint4(Ops::kInf2, Ops::kInf2, Ops::kInf2, Ops::kInf2);
         high[i] = make_uint4(Ops::kNegInf2, Ops::kNegInf2, Ops::kNegInf2, Ops::kNegInf2);
     }
-    if (mine) {
-        src += t0 * src_st[0] + (h0 + head) * src_st[1];
-        dst += (h0 + head) * dst_head;
-        for (int tok = lane; tok < tokens; tok += lanes) {
-            const uint16_t* row = src + tok * src_st[0];
-            uint4 a = *reinterpret_cast<const uint4*>(row + va * 8);
-            uint4 bb = paired ? *reinterpret_cast<const uint4*>(row + vb * 8) : make_uint4(0, 0, 0, 0);
-            bool good = true;
-            if (p.cos) {
-                const long long pos = p.positions ? (long long)p.positions[t0 + tok] : first + tok;
-                good = pos >= 0 && pos < p.table_rows;
-                if (!good) {
-                    report(c, FCS_STATUS_BAD_POSITION);
-                    a = bb = make_uint4(0, 0, 0, 0);
-                } else if (paired) {
-                    const long long at = pos * (p.rotary / 2) + va * 8;
-                    turn_halves<Ops>(a, bb, p.cos + at, p.sin + at);
-                } else if (side_by_side) {
-                    const long long at = pos * (p.rotary / 2) + va * 4;
-                    turn_neighbours<Ops>(a, p.cos + at, p.sin + at);
-                }
-            }
-            if (kind != 2 && !good) continue;
-            uint16_t* out = dst + tok * dst_token;
-            *reinterpret_cast<uint4*>(out + va * 8) = a;
-            if (paired) *reinterpret_cast<uint4*>(out + vb * 8) = bb;
+    for (int tok = mine ? lane : tokens; tok < tokens; tok += lanes) {
+        Turn turn;
+        uint4 a = *reinterpret_cast<const uint4*>(src), bb;
+        if (paired) bb = *reinterpret_cast<const uint4*>(src + apart);
+        if (turn_of(tok, turn)) {
+            apply(turn, a, bb);
+            *reinterpret_cast<uint4*>(dst) = a;
             take_in<Ops>(low[0], high[0], a, a);
-            take_in<Ops>(low[1], high[1], bb, bb);
+            if (paired) {
+                *reinterpret_cast<uint4*>(dst + apart) = bb;
+                take_in<Ops>(low[1], high[1], bb, bb);
+            }
         }
+        src += lanes * src_token;
+        dst += lanes * dst_token;
     }
-    if (kind != 0 || !p.bounds) return;
+    if (!p.bounds) return;
     // the lanes of a head meet, and the first takes in what the page had
     const int busy = min(lanes, tokens);
     if (busy > 1) {
@@ -243,12 +292,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
         }
     }
     if (!mine || lane > 0) return;
-    uint16_t* at = p.bounds + ((long long)page * c.kv_heads + h0 + head) * 2 * D;
+    uint16_t* at = p.bounds + ((long long)page * c.kv_heads + h0 + head) * 2 * D + va * 8;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (i && !paired) break;
-        uint4* lo = reinterpret_cast<uint4*>(at + (i ? vb : va) * 8);
-        uint4* hi = reinterpret_cast<uint4*>(at + D + (i ? vb : va) * 8);
+        uint4* lo = reinterpret_cast<uint4*>(at + i * apart);
+        uint4* hi = reinterpret_cast<uint4*>(at + i * apart + D);
         if (slot0 > 0) take_in<Ops>(low[i], high[i], *lo, *hi);
         *lo = low[i];
         *hi = high[i];
