@@ -85,6 +85,24 @@ static cudaError_t launch(void (*kern)(Params...), dim3 grid, int threads, int s
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+template <typename F>
+static cudaError_t allow_smem(F* kern, int bytes, bool wide_cluster = false) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && wide_cluster) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e;
+}
+
+// Runs `set_up` once per device and instance (`done` is the instance's).
+template <typename F>
+static cudaError_t once_per_device(bool (&done)[64], F set_up) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+    e = set_up();
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+    return e;
+}
+
 // ------------------------------------------------------------------ append
 template <typename Ops>
 static cudaError_t launch_append(int rot, dim3 grid, cudaStream_t stream, const AppendParams& p) {
@@ -202,24 +220,6 @@ static SelectPlan select_plan(const FcsPagedCache* c) {
     s.errors = s.scores + (s.tiles ? (size_t)rows * s.pitch * 4 : 0);
     s.bytes = s.errors + (s.tiles ? (size_t)rows * s.splits * 4 : 0);
     return s;
-}
-
-template <typename F>
-static cudaError_t allow_smem(F* kern, int bytes, bool wide_cluster = false) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && wide_cluster) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e;
-}
-
-// Runs `set_up` once per device and instance (`done` is the instance's).
-template <typename F>
-static cudaError_t once_per_device(bool (&done)[64], F set_up) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
-    e = set_up();
-    if (e == cudaSuccess && dev < 64) done[dev] = true;
-    return e;
 }
 
 template <bool BF16, int DP, int CL>
@@ -362,6 +362,25 @@ static cudaError_t launch_attend_cl(int cl, const CUtensorMap& km, const CUtenso
                      : launch_attend<DP, NT, BF16, 1>(km, vm, p, s);
 }
 
+template <int DP, bool BF16, int CL>
+static cudaError_t launch_shared(const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t stream) {
+    constexpr int STAGES = DP == 128 ? 2 : 3;
+    using L = SharedLayout<DP, STAGES>;
+    auto* kern = attend_shared_kernel<DP, STAGES, BF16, CL>;
+    static bool done[64] = {false};
+    const cudaError_t e = once_per_device(done, [&] { return allow_smem(kern, L::bytes(SHARED_PAGES)); });
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)(CL * ((long long)p.c.tokens / p.tile_tokens + p.c.sequences + 1)), p.c.kv_heads);
+    return launch(kern, grid, SHARED_THREADS, L::bytes(p.c.width), CL, stream, km, vm, p);
+}
+
+template <int DP, bool BF16>
+static cudaError_t launch_shared_cl(int cl, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t s) {
+    return cl == 4   ? launch_shared<DP, BF16, 4>(km, vm, p, s)
+           : cl == 2 ? launch_shared<DP, BF16, 2>(km, vm, p, s)
+                     : launch_shared<DP, BF16, 1>(km, vm, p, s);
+}
+
 static int pool_map(CUtensorMap* m, const FcsPagedCache* c, const void* base, const int64_t* stride) {
     // (the stride of an axis of one entry says nothing; the contiguous one stands in for it)
     int64_t st[3] = {stride[0], stride[1], stride[2]};
@@ -374,6 +393,19 @@ static int pool_map(CUtensorMap* m, const FcsPagedCache* c, const void* base, co
     }
     return make_tensor_map(m, base, c->dtype, c->pages, c->kv_heads, c->page_size, c->dim, st[0], st[1], st[2],
                            c->page_size < TILE_KEYS ? c->page_size : TILE_KEYS);
+}
+
+// CTAs that share a row's keys, up to `most`: the device runs `per_sm` CTAs per SM, rounds of them one after the other, and a CTA
+// costs about a third of a whole row's work beside its share.
+static int cluster_for(long long rows, int per_sm, int most) {
+    const long long slots = (long long)per_sm * num_sms();
+    int best = 1;
+    double least = 1e30;
+    for (int cl = 1; cl <= most; cl *= 2) {
+        const double cost = (double)((rows * cl + slots - 1) / slots) * (1.0 / cl + 0.3);
+        if (cost < least) least = cost, best = cl;
+    }
+    return best;
 }
 
 static int attend(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const int* chosen, int k,
@@ -403,19 +435,29 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     p.q_heads = q_heads;
     p.c_log2 = scale * 1.4426950408889634f;
     p.fill_tail = fill_tail;
-    const int nt = p.group > 8 ? 2 : 1;
-    p.query_tiles = (p.group + 8 * nt - 1) / (8 * nt);
-    // CTAs of a row: as many as the device has room for, two tiles of keys for each at least
-    const long long rows = (long long)cache->tokens * cache->kv_heads * p.query_tiles;
-    const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
-    int cl = 1;
-    while (cl < 8 && rows * cl * 2 <= 2ll * num_sms() && tiles >= 4ll * cl) cl *= 2;
-    if (rows / cache->kv_heads * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
+    const bool wide = cache->dim > 64, bf16 = cache->dtype == FCS_DTYPE_BF16;
     CUtensorMap km, vm;
     if ((rc = pool_map(&km, cache, cache->key_pages, cache->key_stride)) != FCS_OK) return rc;
     if ((rc = pool_map(&vm, cache, cache->value_pages, cache->value_stride)) != FCS_OK) return rc;
-    const bool wide = cache->dim > 64, bf16 = cache->dtype == FCS_DTYPE_BF16;
     cudaError_t e;
+    const long long T = cache->tokens, B = cache->sequences;
+    p.tile_tokens = SHARED_COLS / p.group < 31 ? SHARED_COLS / p.group : 31;
+    if (cache->starts && T >= 2 * B && p.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES) {
+        // several tokens a sequence share what they chose in common
+        const long long ctas = (T / p.tile_tokens > B ? T / p.tile_tokens : B) * cache->kv_heads;
+        const int cl = cluster_for(ctas, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 4);
+        if (4 * (T / p.tile_tokens + B + 1) > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
+        e = wide ? (bf16 ? launch_shared_cl<128, true>(cl, km, vm, p, stream) : launch_shared_cl<128, false>(cl, km, vm, p, stream))
+                 : (bf16 ? launch_shared_cl<64, true>(cl, km, vm, p, stream) : launch_shared_cl<64, false>(cl, km, vm, p, stream));
+        if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "attending failed to launch: %s", cudaGetErrorString(e));
+        return FCS_OK;
+    }
+    const int nt = p.group > 8 ? 2 : 1;
+    p.query_tiles = (p.group + 8 * nt - 1) / (8 * nt);
+    const long long rows = T * cache->kv_heads * p.query_tiles;
+    const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
+    const int cl = cluster_for(rows, 2, tiles >= 16 ? 8 : tiles >= 8 ? 4 : tiles >= 4 ? 2 : 1);     // (two tiles of keys for each CTA at least)
+    if (rows / cache->kv_heads * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
     if (wide)
         e = nt == 1 ? (bf16 ? launch_attend_cl<128, 1, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 1, false>(cl, km, vm, p, stream))
                     : (bf16 ? launch_attend_cl<128, 2, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 2, false>(cl, km, vm, p, stream));

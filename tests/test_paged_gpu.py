@@ -309,6 +309,10 @@ ATTENDS = [
     ([3], [32 * 200], 32, 2, 18, 72, FP16, 150),
     ([1], [64 * 300], 64, 1, 8, 128, FP16, 290),
     ([1] * 260, [1 + 2 * i for i in range(260)], 16, 1, 4, 16, BF16, 3),
+    ([70, 1, 0, 33], [1500, 40, 9, 128 * 5], 64, 2, 8, 128, BF16, 9),
+    ([65], [128 * 12 + 64], 128, 1, 32, 128, FP16, 7),
+    ([40, 3], [900, 16 * 30 + 3], 16, 2, 10, 88, BF16, 20),
+    ([100], [16 * 40], 16, 1, 1, 48, FP16, 11),
 ]
 
 
@@ -404,8 +408,63 @@ def test_attend_with_scores_at_the_ends_of_the_range():
             assert ((got[:, h] - lse[:, h]).abs() <= 72 * 2.0 ** -23 * finite + 2.0 ** -18).all(), (dtype, h)
         assert (out[:, 2] == 0).all() and (got[:, 2] == -math.inf).all()
         assert out[:, 3].isnan().all() and got[:, 3].isnan().all()
-        assert out[:, 4].isnan().all()
+        assert out[:, 4].isnan().all() and (got[:, 4] == math.inf).all()
         status_is(0)
+
+
+@pytest.mark.parametrize("D,P,group", [(128, 64, 4), (64, 16, 1), (96, 128, 8)])
+def test_attend_keeps_the_tokens_of_a_block_apart(D, P, group):
+    """Neighbouring tokens whose lists share pages: values that are not finite reach those that listed their page, and no others;
+    nor do the keys behind a token, or a page that another token listed twice."""
+    import flash_colsum_b200 as fc
+    a = Batch(21, [23], [P * 9 + 5], P, 2, 2 * group, D, BF16)
+    query, pools = a.rows(2 * group), [a.pool(), a.pool()]
+    pages = torch.full((a.T, 2, 6), -1, dtype=torch.int32)
+    for t in range(a.T):
+        for h in range(2):
+            order = torch.randperm(9, generator=a.g)[:5].int()
+            pages[t, h, :5] = order
+    for kind in ("nan in a page", "inf in keys and values", "nan in a later token", "twice"):
+        k, v, lists = pools[0].clone(), pools[1].clone(), pages.clone()
+        if kind == "nan in a page":
+            v[int(a.table[0, 3]), :, P - 1, 2] = math.nan
+        elif kind == "inf in keys and values":
+            v[int(a.table[0, 4]), 1, 0, :] = math.inf
+            k[int(a.table[0, 5]), 0, 3, 1] = math.inf
+        elif kind == "nan in a later token":          # the block's own page, which all of it lists
+            lists[:, :, 5] = 9 if P > 23 else lists[:, :, 5]
+            at = a.lens[0] - 2
+            v[int(a.table[0, at // P]), :, int(at) % P, 0] = math.nan
+        else:
+            lists[11, 0, 5] = lists[11, 0, 1]
+            lists[4, 1, 0:3] = 2
+        want, lse, spread, reach = attention(query, k, v, a.table, a.lens, a.starts, lists, D ** -0.5)
+        out, got = fc.attend_pages(*on_gpu(query, k, v, a.table, a.lens, lists), starts=a.starts.cuda(), return_lse=True)
+        out, got = out.cpu().double(), got.cpu().double()
+        assert torch.equal(out.isfinite(), want.isfinite())
+        fine = want.isfinite()
+        room = attend_room(BF16, D, 6 * P, want, spread, reach)
+        assert ((out - want).abs() <= room)[fine].all()
+        some = lse.isfinite()
+        assert torch.equal(got[~some].isnan(), lse[~some].isnan())
+        assert torch.equal(got == math.inf, lse == math.inf)
+        assert ((got - lse).abs() <= (D + 8) * 2.0 ** -23 * reach + 2.0 ** -18 + lse.abs() * 2.0 ** -22)[some].all()
+    status_is(0)
+
+
+@pytest.mark.parametrize("width", [8192, 8193])
+def test_attend_of_blocks_under_a_wide_table(width):
+    """On both sides of the widest table that tokens share their pages under."""
+    import flash_colsum_b200 as fc
+    a = Batch(22, [9, 30], [16 * 50, 16 * 70 + 1], 16, 2, 4, 64, FP16, width=width, tail=3)
+    query, pools = a.rows(4), [a.pool(), a.pool()]
+    pages = listed_pages(a, 8)
+    pages[2, 0, 0], pages[2, 1, 1] = 8192, 2 ** 31 - 1            # behind the token
+    want, lse, spread, reach = attention(query, *pools, a.table, a.lens, a.starts, pages, 0.125)
+    out = fc.attend_pages(*on_gpu(query, *pools, a.table, a.lens, pages), starts=a.starts.cuda())
+    assert ((out.cpu().double() - want).abs() <= attend_room(FP16, 64, 128, want, spread, reach)).all()
+    assert (out[39:] == 0).all()
+    status_is(0)
 
 
 def test_attend_reads_nothing_from_pages_that_the_table_lacks():
