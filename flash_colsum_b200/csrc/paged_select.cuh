@@ -151,11 +151,10 @@ struct ExactScores {
     }
 };
 
-// Pages whose scores are too close to tell, up to 32 of them (shared memory of a team).
+// Pages around the border, up to 32 of them (shared memory of a team).
 struct CloseList {
     unsigned long long key[32];
     int page[32];
-    uint32_t n;
 };
 
 // ---- who chooses for a row: a block, or a warp.  A thread holds the keys of E consecutive pages (a block goes over more than
@@ -186,9 +185,8 @@ __device__ __forceinline__ uint32_t warp_upto(uint32_t n) {       // inclusive s
 
 template <int NT, int E>
 struct BlockTeam {
-    static constexpr int SIZE = NT, RUN = E, BINS = 4 * NT;
+    static constexpr int SIZE = NT, RUN = E;
     const float* scores;
-    uint32_t* bins;              // shared: [BINS], zeros at first
     CloseList* close;            // shared
     uint32_t* room;              // shared: [2][3 * NT / 32]
     int turn = 0;
@@ -237,31 +235,12 @@ struct BlockTeam {
         }
         return sum;
     }
-    // The bin that the `need`-th entry from the top is in, what is above it, and its count.
-    __device__ void locate(uint32_t need, uint32_t& above, uint32_t& bin, uint32_t& count) {
-        const uint32_t at = BINS - 4 * (threadIdx.x + 1);
-        const uint4 q = *reinterpret_cast<const uint4*>(&bins[at]);
-        uint32_t total;
-        const uint32_t from = before(q.x + q.y + q.z + q.w, total);
-        if (from < need && need <= from + q.x + q.y + q.z + q.w) {
-            const uint32_t a3 = from + q.w, a2 = a3 + q.z, a1 = a2 + q.y;
-            const int i = need <= a3 ? 3 : need <= a2 ? 2 : need <= a1 ? 1 : 0;
-            close->n = at + i;                 // (free until a list is made)
-            close->page[0] = (int)(i == 3 ? from : i == 2 ? a3 : i == 1 ? a2 : a1);
-            close->page[1] = (int)(i == 3 ? q.w : i == 2 ? q.z : i == 1 ? q.y : q.x);
-        }
-        __syncthreads();
-        bin = close->n;
-        above = (uint32_t)close->page[0];
-        count = (uint32_t)close->page[1];
-    }
 };
 
 template <int E>
 struct WarpTeam {
-    static constexpr int SIZE = 32, RUN = E, BINS = 256;
+    static constexpr int SIZE = 32, RUN = E;
     const float* scores;
-    uint32_t* bins;              // shared, the warp's own: [BINS], zeros at first
     CloseList* close;            // shared, the warp's own
     uint32_t keys[E];
     __device__ int rank() const { return threadIdx.x & 31; }
@@ -281,34 +260,6 @@ struct WarpTeam {
         total = __shfl_sync(0xffffffffu, upto, 31);
         return upto - n;
     }
-    __device__ void locate(uint32_t need, uint32_t& above, uint32_t& bin, uint32_t& count) const {
-        constexpr int PER = BINS / 32;
-        const int lane = rank();
-        uint32_t n[PER], sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(&bins[BINS - PER * (lane + 1) + i]);
-            n[i] = q.x, n[i + 1] = q.y, n[i + 2] = q.z, n[i + 3] = q.w;
-            sum += q.x + q.y + q.z + q.w;
-        }
-        const uint32_t upto = warp_upto(sum);
-        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= need)) - 1;
-        above = upto - sum;
-        bin = count = 0;
-        bool open = true;
-#pragma unroll
-        for (int i = PER - 1; i >= 0; --i) {
-            if (open && above + n[i] >= need) {
-                open = false;
-                bin = BINS - PER * (lane + 1) + i;
-                count = n[i];
-            }
-            if (open) above += n[i];
-        }
-        above = __shfl_sync(0xffffffffu, above, owner);
-        bin = __shfl_sync(0xffffffffu, bin, owner);
-        count = __shfl_sync(0xffffffffu, count, owner);
-    }
 };
 
 struct Sum {
@@ -320,34 +271,8 @@ struct Largest {
     __device__ uint32_t warp(uint32_t v) const { return __reduce_max_sync(0xffffffffu, v); }
 };
 
-// The `need`-th largest key of a row, or a key that as many as `need` reach: then `clean` is set.  Keys are in low .. high, more
-// than `need` of them.  A histogram over the range, and again over the bin that holds the place, until a bin is wanted whole.
-template <typename Team>
-__device__ uint32_t kth_key(const Row& r, Team& team, uint32_t need, uint32_t low, uint32_t high, bool& clean) {
-    constexpr int BINS = Team::BINS;
-    while (true) {
-        const int width = 32 - __clz(high - low);      // bits of the range
-        const int shift = max(0, width - (31 - __clz(BINS)));
-        team.tiles(r, [&](int) {
-#pragma unroll
-            for (int j = 0; j < Team::RUN; ++j)
-                if (team.keys[j] >= low && team.keys[j] <= high) atomicAdd(&team.bins[(team.keys[j] - low) >> shift], 1u);
-        });
-        team.sync();
-        uint32_t above, bin, count;
-        team.locate(need, above, bin, count);
-        need -= above;
-        low += bin << shift;
-        clean = count == need;
-        if (clean || shift == 0) return low;
-        high = low + ((1u << shift) - 1);
-        team.sync();                                   // (all have read the bins)
-        for (int i = team.rank() * 4; i < BINS; i += Team::SIZE * 4) *reinterpret_cast<uint4*>(&team.bins[i]) = make_uint4(0, 0, 0, 0);
-        team.sync();
-    }
-}
-
-// The same over 64-bit keys in low .. high - 1 that `each` goes over, three guesses at a time.
+// The `need`-th largest of the 64-bit keys that `each` goes over -- at least `need` are >= low, fewer >= high --, or a key that as
+// many as `need` reach: then `clean` is set.
 template <typename Team, typename Each>
 __device__ unsigned long long kth_wide_key(Team& team, uint32_t need, unsigned long long low, unsigned long long high, bool& clean,
                                            Each each) {
@@ -376,15 +301,34 @@ __device__ unsigned long long kth_wide_key(Team& team, uint32_t need, unsigned l
 
 // Chooses the pages of a row and writes them.  `ends`: the largest key and the complement of the smallest, or zeros.  `error`: E.
 // `exact`: the row's memory for sums in 64 bits.
+//
+// The border is looked for with three guesses at a time, which a straight line through the logarithms of the counts places: the
+// tail of a sum of many terms falls about so.  When at most 24 pages are left, they and those within the error of them are listed,
+// and a warp ranks the list -- each warp for itself.  Where more are left (equal pages, no finite error) 64 bits decide about all.
+// [rows of 2048 and 512 pages: three rounds, where halving takes seven and a histogram of 1024 bins two of twice the time]
 template <bool BF16, typename Team>
 __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t (&ends)[3], float error, double* exact, int* out) {
     constexpr int E = Team::RUN;
     uint32_t(&keys)[E] = team.keys;
+    const int lane = threadIdx.x & 31;
     team.load(r, 0);
-    // keys above `sure` are chosen, keys from `open` on may be
-    uint32_t sure = 0xffffffffu, open = 0xffffffffu;
-    unsigned long long bar = ~0ull;       // of the latter: 64-bit keys above `bar`, and the first `equal` at it
-    uint32_t equal = 0, picked = 0;       // or of a list of them, the picked
+    // chosen: keys from `high` on, and of those from `low` on: the listed ones that are `picked`, or (wide) those whose 64-bit key is
+    // above `bar`, and the first `equal` at it
+    uint32_t low = 0xffffffffu, high = 0xffffffffu, picked = 0, equal = 0;
+    unsigned long long bar = 0;
+    bool wide = false;
+    auto count = [&](uint32_t m0, uint32_t m1, uint32_t m2, uint32_t (&n)[3]) {
+        n[0] = n[1] = n[2] = 0;
+        team.tiles(r, [&](int) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                n[0] += keys[j] >= m0;
+                n[1] += keys[j] >= m1;
+                n[2] += keys[j] >= m2;
+            }
+        });
+        team.reduce(n, Sum());
+    };
     if (r.need > 0) {
         if (ends[0] == 0) {
             team.tiles(r, [&](int) {
@@ -396,123 +340,162 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
             });
             team.reduce(ends, Largest());
         }
-        bool clean;
-        uint32_t kth = kth_key(r, team, r.need, ~ends[1], ends[0], clean);
-        bool apart = false;
-        if (clean) {                      // the smallest above, the largest below
-            uint32_t near[3] = {0, 0, 0};
-            team.tiles(r, [&](int) {
-#pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    if (keys[j] >= kth) near[0] = max(near[0], ~keys[j]);
-                    else near[1] = max(near[1], keys[j]);
-                }
-            });
-            team.reduce(near, Largest());
-            const uint32_t above = ~near[0];
-            apart = value_of(above) - value_of(near[1]) > 2.5f * error;
-            if (apart) sure = above - 1;
-            kth = above;
+        low = ~ends[1];
+        high = ends[0] + 1;
+        const bool known = error < INFINITY;
+        // at least `need` keys are >= low, fewer are >= high
+        uint32_t at_low = (uint32_t)(r.hi - r.lo), at_high = 0, n[3];
+        auto narrow = [&](uint32_t m0, uint32_t m1, uint32_t m2) {
+            count(m0, m1, m2, n);
+            if (n[2] >= r.need) low = m2, at_low = n[2];
+            else if (n[1] >= r.need) low = m1, at_low = n[1], high = m2, at_high = n[2];
+            else if (n[0] >= r.need) low = m0, at_low = n[0], high = m1, at_high = n[1];
+            else high = m0, at_high = n[0];
+        };
+        while (known && high - low > 1 && at_low - at_high > 24) {
+            const float top = __log2f((float)at_low + 0.5f), bottom = __log2f((float)at_high + 0.5f);
+            const float f = (top - __log2f((float)r.need + 0.5f)) / (top - bottom), d = (float)(high - low);
+            const uint32_t last = high - low - 1;
+            auto guess = [&](float part) { return low + max(1u, min(last, (uint32_t)(part * d))); };
+            narrow(guess(0.5f * f), guess(f), guess(0.5f + 0.5f * f));
         }
-        if (!apart) {
-            // (2.5: the sums below are rounded, too)
-            const float t = value_of(kth);
-            const bool known = error < INFINITY;
-            sure = known ? key_of(t + 2.5f * error) : 0xffffffffu;
-            open = known ? key_of(t - 2.5f * error) : 1u;
-            uint32_t n[3] = {0, 0, 0};
-            team.tiles(r, [&](int) {
+        bool listed = false;
+        uint32_t above = 0;
+        if (known) {     // as far as the errors reach (2.5: the sums here are rounded, too)
+            const uint32_t from = key_of(value_of(low) - 2.6f * error);
+            const uint32_t upto = high > ends[0] ? high : max(high, key_of(value_of(high) + 2.6f * error) + 1);
+            count(from, upto, upto, n);
+            listed = n[0] - n[1] <= 32;
+            if (listed) low = from, high = upto, above = n[1];
+        }
+        if (listed) {
+            const int m = (int)(n[0] - n[1]);
+            const uint32_t want = r.need - above;
+            uint32_t slot = 0, total;
+            team.tiles(r, [&](int i) {
+                uint32_t in = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (keys[j] >= low && keys[j] < high) in |= 1u << j;
+                uint32_t at = slot + team.before(__popc(in), total);
+                slot += total;
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (in >> j & 1u) {
+                        team.close->key[at] = keys[j];
+                        team.close->page[at++] = i + j;
+                    }
+            });
+            team.sync();
+            const uint32_t key = lane < m ? (uint32_t)team.close->key[lane] : 0u;
+            uint32_t ahead = 0;
+            for (int i = 0; i < m; ++i) {
+                const uint32_t other = __shfl_sync(0xffffffffu, key, i);
+                ahead += other > key || (other == key && i < lane);
+            }
+            const float v = value_of(key), t = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, lane < m && ahead + 1 == want)) - 1);
+            const uint32_t sure = __ballot_sync(0xffffffffu, lane < m && v > t + 2.5f * error);
+            const uint32_t near = __ballot_sync(0xffffffffu, lane < m && !(v > t + 2.5f * error) && v >= t - 2.5f * error);
+            const uint32_t left = want - __popc(sure);
+            picked = sure | near;
+            if ((int)left < __popc(near)) {
+                const ExactScores<BF16> score(p, r);
+                const int warp = Team::SIZE > 32 ? threadIdx.x >> 5 : 0;
+                team.sync();               // (the keys have been read)
+                uint32_t todo = near;
+                for (int i = 0; todo; ++i, todo &= todo - 1)
+                    if (i % (Team::SIZE / 32) == warp) {
+                        const int at = __ffs(todo) - 1;
+                        const double s = score(p, r, team.close->page[at]);
+                        if (lane == 0) team.close->key[at] = key_of(s);
+                    }
+                team.sync();
+                const unsigned long long mine = team.close->key[lane < m ? lane : 0];
+                ahead = 0;
+                for (todo = near; todo; todo &= todo - 1) {
+                    const int i = __ffs(todo) - 1;
+                    const unsigned long long other = team.close->key[i];
+                    ahead += other > mine || (other == mine && i < lane);
+                }
+                picked = sure | __ballot_sync(0xffffffffu, (near >> lane & 1u) && ahead < left);
+            }
+        } else {
+            wide = true;
+            while (known && high - low > 1) {
+                const uint32_t d = high - low, quarter = max(1u, d / 4);
+                narrow(low + quarter, low + max(1u, d / 2), low + max(1u, d / 4 * 3));
+            }
+            const float t = value_of(low);       // the need-th largest
+            low = known ? key_of(t - 2.5f * error) : 1u;
+            high = known ? key_of(t + 2.5f * error) + 1 : 0xffffffffu;
+            count(low, high, high, n);
+            const uint32_t left = r.need - n[1];
+            const ExactScores<BF16> score(p, r);
+            team.tiles(r, [&](int i) {
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    n[0] += keys[j] > sure;
-                    n[1] += keys[j] >= open && keys[j] <= sure;
+                    uint32_t todo = __ballot_sync(0xffffffffu, keys[j] >= low && keys[j] < high);
+                    while (todo) {
+                        const int src = __ffs(todo) - 1;
+                        todo &= todo - 1;
+                        const int page = __shfl_sync(0xffffffffu, i, src) + j;
+                        const double s = score(p, r, page);
+                        if (lane == src) exact[page] = s;
+                    }
                 }
             });
-            team.reduce(n, Sum());
-            const uint32_t left = r.need - n[0];
-            const bool listed = n[1] <= 32;
-            if (n[1] == left) {           // all of them
-                bar = 0;
-            } else {
-                if (team.rank() == 0) team.close->n = 0;
-                team.sync();
-                const ExactScores<BF16> score(p, r);
+            team.sync();
+            auto over = [&](auto f) {
                 team.tiles(r, [&](int i) {
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        uint32_t todo = __ballot_sync(0xffffffffu, keys[j] >= open && keys[j] <= sure);
-                        while (todo) {
-                            const int src = __ffs(todo) - 1;
-                            todo &= todo - 1;
-                            const int page = __shfl_sync(0xffffffffu, i, src) + j;
-                            const double s = score(p, r, page);
-                            if ((int)(threadIdx.x & 31) == src) {
-                                if (listed) {
-                                    const uint32_t at = atomicAdd(&team.close->n, 1u);
-                                    team.close->key[at] = key_of(s);
-                                    team.close->page[at] = page;
-                                } else {
-                                    exact[page] = s;
-                                }
-                            }
-                        }
-                    }
+                    for (int j = 0; j < E; ++j)
+                        if (keys[j] >= low && keys[j] < high) f(key_of(exact[i + j]));
                 });
-                team.sync();
-            }
-            if (n[1] != left && listed) {       // every warp for itself: how many are before a lane's page
-                const int lane = threadIdx.x & 31, m = (int)n[1];
-                const unsigned long long key = lane < m ? team.close->key[lane] : 0ull;
-                const int page = lane < m ? team.close->page[lane] : 0;
-                uint32_t ahead = 0;
-                for (int i = 0; i < m; ++i) {
-                    const unsigned long long other = team.close->key[i];
-                    ahead += other > key || (other == key && team.close->page[i] < page);
-                }
-                picked = __ballot_sync(0xffffffffu, lane < m && ahead < left);
-            } else if (n[1] != left) {
-                auto over_open = [&](auto count) {
-                    team.tiles(r, [&](int i) {
-#pragma unroll
-                        for (int j = 0; j < E; ++j)
-                            if (keys[j] >= open && keys[j] <= sure) count(key_of(exact[i + j]));
-                    });
-                };
+            };
+            if (left == n[0] - n[1]) {           // all of them
+                bar = 0;
+            } else {
                 // (within E of sums that are within 2.5 E of t)
+                bool clean;
                 bar = kth_wide_key(team, left, known ? key_of((double)t - 4.0 * error) : 0ull,
-                                   known ? key_of((double)t + 4.0 * error) + 1 : ~0ull, clean, over_open);
+                                   known ? key_of((double)t + 4.0 * error) + 1 : ~0ull, clean, over);
                 if (clean) {
                     bar -= 1;
                 } else {
-                    uint32_t above[3] = {0, 0, 0};
-                    over_open([&](unsigned long long key) { above[0] += key > bar; });
-                    team.reduce(above, Sum());
-                    equal = left - above[0];
+                    uint32_t higher[3] = {0, 0, 0};
+                    over([&](unsigned long long key) { higher[0] += key > bar; });
+                    team.reduce(higher, Sum());
+                    equal = left - higher[0];
                 }
             }
         }
     }
-    uint32_t place = 0, equal_before = 0, total;
+    uint32_t place = 0, slot = 0, equal_before = 0, total;
     team.tiles(r, [&](int i) {
-        uint32_t taken = 0, same = 0;     // a bit per page of the run
+        uint32_t taken = 0, in = 0, same = 0;     // a bit per page of the run
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            bool take = i + j < r.pages && (keys[j] == 0 || keys[j] > sure);
-            if (keys[j] >= open && keys[j] <= sure) {
-                if (picked) {
-                    for (uint32_t left = picked; left; left &= left - 1) take |= team.close->page[__ffs(left) - 1] == i + j;
-                } else {
-                    const unsigned long long wide = bar == 0 ? 1ull : key_of(exact[i + j]);
-                    take = wide > bar;
-                    if (wide == bar) same |= 1u << j;
-                }
-            }
-            if (take) taken |= 1u << j;
+            if (i + j < r.pages && (keys[j] == 0 || keys[j] >= high)) taken |= 1u << j;
+            if (keys[j] >= low && keys[j] < high) in |= 1u << j;
         }
-        if (equal > 0) {                  // (the same for all)
-            uint32_t rank = equal_before + team.before(__popc(same), total);
-            equal_before += total;
-            for (; same && rank < equal; ++rank, same &= same - 1) taken |= same & -same;
+        if (wide) {                               // (the same for all)
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (in >> j & 1u) {
+                    const unsigned long long key = key_of(exact[i + j]);
+                    if (key > bar) taken |= 1u << j;
+                    if (key == bar) same |= 1u << j;
+                }
+            if (equal > 0) {
+                uint32_t rank = equal_before + team.before(__popc(same), total);
+                equal_before += total;
+                for (; same && rank < equal; ++rank, same &= same - 1) taken |= same & -same;
+            }
+        } else {
+            uint32_t at = slot + team.before(__popc(in), total);
+            slot += total;
+            for (; in; ++at, in &= in - 1)
+                if (picked >> at & 1u) taken |= in & -in;
         }
         uint32_t at = place + team.before(__popc(taken), total);
         for (; taken; ++at, taken &= taken - 1)
@@ -551,7 +534,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     __shared__ float warp_size[WARPS], warp_most[WARPS];
     __shared__ uint32_t room[2 * 3 * WARPS];
     __shared__ CloseList close;
-    __shared__ __align__(16) uint32_t bins[RowTeam::BINS];
     __shared__ __align__(16) uint16_t parts[4][2 * DP];       // what 16 bits hold, the rest of that and the rest's, zeros
     if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     grid_dependency_wait();
@@ -589,7 +571,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     } else if (lane == 0) {
         warp_size[warp] = warp_most[warp] = 0.f;
     }
-    *reinterpret_cast<uint4*>(&bins[tid * 4]) = make_uint4(0, 0, 0, 0);
     Row r = {};
     if (b < c.sequences) r.set(p, t, h, b, pos);
     int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
@@ -707,7 +688,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     }
     size = __shfl_sync(0xffffffffu, size, 0);
     most = __shfl_sync(0xffffffffu, most, 0);
-    RowTeam team{row_scores, bins, &close, room};
+    RowTeam team{row_scores, &close, room};
     const float error = score_error<BF16>(p, size, most, __uint_as_float(ends[2]), CHUNKS + 3, 3);
     choose<BF16>(p, r, team, ends, error, p.exact + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch, out);
 }
@@ -756,14 +737,16 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
     const int my_row = tid >> 2, my_vec = tid & 3;       // four threads a row
     {
         float size = 0.f, most = 0.f;
+#pragma unroll 2
         for (int v = my_vec; v < D / 8; v += 4) {
             float n[8], s[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) n[i] = s[i] = 0.f;
             if (my_row < tokens) {
                 const uint16_t* q = p.query + (t_first + my_row) * p.query_st[0] + (long long)h * p.group * p.query_st[1] + v * 8;
-                for (int g = 0; g < p.group; ++g, q += p.query_st[1]) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(q);
+#pragma unroll 4
+                for (int g = 0; g < p.group; ++g) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(q + g * p.query_st[1]);
                     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -886,10 +869,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_con
     typedef BlockTeam<CHOOSE_THREADS, 16> Block;
     typedef WarpTeam<(E > 0 ? E : 4)> Warp;
     __shared__ uint32_t room[2 * 3 * CHOOSE_THREADS / 32];
-    __shared__ __align__(16) uint32_t bins[E > 0 ? ROWS * Warp::BINS : Block::BINS];
     __shared__ CloseList close[ROWS];
-    for (int i = threadIdx.x; i < (int)(sizeof(bins) / 4); i += CHOOSE_THREADS) bins[i] = 0;
-    __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
     const Batch& c = p.c;
@@ -916,10 +896,10 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_con
     if (!(error < INFINITY)) error = INFINITY;
     uint32_t ends[3] = {0, 0, 0};
     if constexpr (E > 0) {
-        Warp team{scores, bins + (threadIdx.x >> 5) * Warp::BINS, &close[threadIdx.x >> 5]};
+        Warp team{scores, &close[threadIdx.x >> 5]};
         choose<BF16>(p, r, team, ends, error, exact, out);
     } else {
-        Block team{scores, bins, close, room};
+        Block team{scores, close, room};
         choose<BF16>(p, r, team, ends, error, exact, out);
     }
 }
