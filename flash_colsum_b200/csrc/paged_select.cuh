@@ -521,13 +521,19 @@ __device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row&
 constexpr int ROW_THREADS = 256;
 typedef BlockTeam<ROW_THREADS, 8> RowTeam;
 
-// grid: (CL * tokens, kv heads); shared memory: `pitch` scores.  A warp takes 16 pages at a time as the rows of a matrix
-// instruction straight from memory -- a lane loads eight neighbouring features, which serve as those that the instruction wants of
-// it, in the order that the parts are given in as well.  The parts' two pieces are two of its eight columns.
+// grid: (CL * tokens, kv heads); shared memory: row_smem.  A warp takes 16 pages at a time, whose bounds bulk copies bring -- it
+// asks for the next 16 when it has read these -- as the rows of a matrix instruction: a lane reads eight neighbouring features,
+// which serve as those that the instruction wants of it, in the order that the parts are given in as well.  The parts' three
+// pieces are three of its eight columns.  (Loads into registers in place of the copies: 32 rows of 256 to 512 pages 26.5 us.)
+__host__ __device__ constexpr int row_block_bytes(int dim) { return 16 * (4 * dim + 16); }       // (16: no bank twice)
+inline int row_smem(int dim, int pitch) { return ROW_THREADS / 32 * row_block_bytes(dim) + 4 * pitch; }
+
 template <bool BF16, int DP, int CL>
-__global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(ROW_THREADS, 3) select_row_kernel(const __grid_constant__ SelectParams p) {
     constexpr int CHUNKS = DP / 16;               // 32 of the 2 D features
-    extern __shared__ __align__(16) float row_scores[];
+    extern __shared__ __align__(16) uint8_t row_smem_raw[];
+    __shared__ __align__(8) unsigned long long arrived[ROW_THREADS / 32];
+    __shared__ int abort_flag;
     constexpr int WARPS = ROW_THREADS / 32;
     __shared__ uint32_t of_cta[3][CL];            // the largest key, the complement of the smallest, the reach
     __shared__ uint32_t of_warp[3][WARPS];
@@ -535,12 +541,19 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     __shared__ uint32_t room[2 * 3 * WARPS];
     __shared__ CloseList close;
     __shared__ __align__(16) uint16_t parts[4][2 * DP];       // what 16 bits hold, the rest of that and the rest's, zeros
+    if (threadIdx.x % 32 == 0) mbar_init(smem_u32(&arrived[threadIdx.x / 32]), 1);
+    if (threadIdx.x == 0) abort_flag = 0;
+    mbar_fence_init();
     if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     grid_dependency_wait();
     grid_launch_dependents();
     const Batch& c = p.c;
     const int D = c.dim, h = blockIdx.y, rank = (int)(blockIdx.x % CL), t = p.t0 + (int)(blockIdx.x / CL);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row_bytes = 4 * D + 16;
+    uint8_t* const block = row_smem_raw + warp * row_block_bytes(D);
+    float* const row_scores = reinterpret_cast<float*>(row_smem_raw + WARPS * row_block_bytes(D));
+    const uint32_t bar = smem_u32(&arrived[warp]);
     const int b = sequence_of(c, t);
     const long long pos = b < c.sequences ? position_of(c, b, t) : -1;
 
@@ -582,7 +595,21 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     const int per = (r.hi - r.lo + CL - 1) / CL, begin = r.lo + rank * per, end = min(r.hi, begin + per);
     const int* table = c.table + b * c.table_ld;
     int base = begin + warp * 16;
-    int entry = base + (lane & 15) < end ? table[base + (lane & 15)] : -1;
+    // This warp's next 16 pages; whether each is one of the pools'.  (For one that is not, page 0 stands in.)
+    auto ask = [&](int first, int entry) {
+        const int n = min(16, end - first);
+        if (n <= 0) return;
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * 4 * D));
+        __syncwarp();
+        if (lane < n) {
+            const int page = entry >= 0 && entry < c.pages ? entry : 0;
+            bulk_load(smem_u32(block + lane * row_bytes), p.bounds + ((long long)page * c.kv_heads + h) * 2 * D, 4 * D, bar);
+        }
+    };
+    auto entry_of = [&](int first) { return lane < 16 && first + lane < end ? table[first + lane] : -1; };
+    int entry = entry_of(base);
+    __syncwarp();
+    ask(base, entry);
     uint32_t high_bits = 0, low_bits = 0x80008000u;       // the largest bit patterns, as unsigned and as signed
     bool lacking = false;
     __syncthreads();
@@ -592,43 +619,38 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
     const int row = lane >> 2, col = lane & 3;
     const uint16_t* columns = parts[min(row, 3)] + col * 8;
     uint32_t ends[3] = {0, 0, 0};
+    uint32_t phase = 0;
     while (base < end) {
-        const int page0 = __shfl_sync(0xffffffffu, entry, row), page1 = __shfl_sync(0xffffffffu, entry, row + 8);
-        const bool there0 = page0 >= 0 && page0 < c.pages, there1 = page1 >= 0 && page1 < c.pages;
-        const uint16_t* at0 = p.bounds + ((long long)(there0 ? page0 : 0) * c.kv_heads + h) * 2 * D + col * 8;
-        const uint16_t* at1 = p.bounds + ((long long)(there1 ? page1 : 0) * c.kv_heads + h) * 2 * D + col * 8;
-        const int next = base + ROW_THREADS / 32 * 16;
-        entry = next + (lane & 15) < end ? table[next + (lane & 15)] : -1;
+        const int next = base + WARPS * 16;
+        const int ahead = entry_of(next);
+        if (!mbar_wait(bar, phase, &abort_flag, c.status, FCS_STATUS_WAIT_CONSUMER)) break;
+        phase ^= 1;
+        const bool in0 = base + row < end, in1 = base + row + 8 < end;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s0 = 0; s0 < CHUNKS; s0 += 4) {
-            uint4 w0[4], w1[4];
+        for (int s = 0; s < CHUNKS; ++s) {
+            const bool in = s * 32 + col * 8 < 2 * D;
+            const uint8_t* at = block + row * row_bytes + col * 16 + s * 64;
+            const uint4 w0 = in0 && in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+            const uint4 w1 = in1 && in ? *reinterpret_cast<const uint4*>(at + 8 * row_bytes) : make_uint4(0, 0, 0, 0);
+            const uint4 f = *reinterpret_cast<const uint4*>(columns + s * 32);
+            // (every instruction starts from zero: see score_error)
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t a0[4] = {w0.x, w1.x, w0.y, w1.y}, a1[4] = {w0.z, w1.z, w0.w, w1.w};
+            mma16816<BF16>(x, a0, f.x, f.y);
+            mma16816<BF16>(y, a1, f.z, f.w);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bool in = (s0 + s) * 32 + col * 8 < 2 * D;
-                w0[s] = there0 && in ? *reinterpret_cast<const uint4*>(at0 + (s0 + s) * 32) : make_uint4(0, 0, 0, 0);
-                w1[s] = there1 && in ? *reinterpret_cast<const uint4*>(at1 + (s0 + s) * 32) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const uint4 f = *reinterpret_cast<const uint4*>(columns + (s0 + s) * 32);
-                // (every instruction starts from zero: see score_error)
-                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-                const uint32_t a0[4] = {w0[s].x, w1[s].x, w0[s].y, w1[s].y}, a1[4] = {w0[s].z, w1[s].z, w0[s].w, w1[s].w};
-                mma16816<BF16>(x, a0, f.x, f.y);
-                mma16816<BF16>(y, a1, f.z, f.w);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] += x[i] + y[i];
-                high_bits = __vimax3_u16x2(high_bits, w0[s].x, w0[s].y);
-                high_bits = __vimax3_u16x2(high_bits, w0[s].z, w0[s].w);
-                high_bits = __vimax3_u16x2(high_bits, w1[s].x, w1[s].y);
-                high_bits = __vimax3_u16x2(high_bits, w1[s].z, w1[s].w);
-                low_bits = __vimax3_s16x2(low_bits, w0[s].x, w0[s].y);
-                low_bits = __vimax3_s16x2(low_bits, w0[s].z, w0[s].w);
-                low_bits = __vimax3_s16x2(low_bits, w1[s].x, w1[s].y);
-                low_bits = __vimax3_s16x2(low_bits, w1[s].z, w1[s].w);
-            }
+            for (int i = 0; i < 4; ++i) acc[i] += x[i] + y[i];
+            high_bits = __vimax3_u16x2(__vimax3_u16x2(high_bits, w0.x, w0.y), w0.z, w0.w);
+            high_bits = __vimax3_u16x2(__vimax3_u16x2(high_bits, w1.x, w1.y), w1.z, w1.w);
+            low_bits = __vimax3_s16x2(__vimax3_s16x2(low_bits, w0.x, w0.y), w0.z, w0.w);
+            low_bits = __vimax3_s16x2(__vimax3_s16x2(low_bits, w1.x, w1.y), w1.z, w1.w);
         }
+        __syncwarp();
+        ask(next, ahead);
+        const int page0 = __shfl_sync(0xffffffffu, entry, row), page1 = __shfl_sync(0xffffffffu, entry, row + 8);
+        const bool there0 = page0 >= 0 && page0 < c.pages, there1 = page1 >= 0 && page1 < c.pages;
+        entry = ahead;
         // columns 0 to 2 together are the score; lane 4 i has 0 and 1 of pages i and i + 8, lane 4 i + 1 has 2
         const float third0 = __shfl_down_sync(0xffffffffu, acc[0], 1), third1 = __shfl_down_sync(0xffffffffu, acc[2], 1);
         const float second = __shfl_up_sync(0xffffffffu, (acc[2] + acc[3]) + third1, 1);
@@ -648,6 +670,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) select_row_kernel(const __grid
         __syncwarp();
         base = next;
     }
+    if (abort_flag) __nanosleep(100000);       // (copies of a warp that gave up may still be landing)
     if (lacking) report(c, FCS_STATUS_BAD_PAGE);
     // (the reach is not negative, or NaN: its bits are in order)
     ends[2] = __float_as_uint(reach_of<BF16>(high_bits, low_bits));

@@ -186,7 +186,7 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
 }
 
 // ------------------------------------------------------------------ select
-constexpr int ROW_PAGES = 51200;       // scores that a CTA's shared memory holds
+constexpr int ROW_PAGES = 32768;       // scores that a CTA's shared memory holds beside its pages
 
 // Scores of a row, with a place behind the last.
 static long long select_pitch(const FcsPagedCache* c) { return (c->table_width + 4ll) & ~3ll; }
@@ -225,9 +225,9 @@ static SelectPlan select_plan(const FcsPagedCache* c) {
 template <bool BF16, int DP, int CL>
 static cudaError_t launch_select_row(const SelectParams& p, unsigned tokens, cudaStream_t stream) {
     static bool done[64] = {false};
-    const cudaError_t e = once_per_device(done, [] { return allow_smem(select_row_kernel<BF16, DP, CL>, ROW_PAGES * 4, CL > 8); });
+    const cudaError_t e = once_per_device(done, [] { return allow_smem(select_row_kernel<BF16, DP, CL>, row_smem(DP, ROW_PAGES), CL > 8); });
     if (e != cudaSuccess) return e;
-    return launch(select_row_kernel<BF16, DP, CL>, dim3(CL * tokens, p.c.kv_heads), ROW_THREADS, p.pitch * 4, CL, stream, p);
+    return launch(select_row_kernel<BF16, DP, CL>, dim3(CL * tokens, p.c.kv_heads), ROW_THREADS, row_smem(p.c.dim, p.pitch), CL, stream, p);
 }
 
 template <bool BF16, int DP>
@@ -250,7 +250,7 @@ static bool clusters_of_sixteen_fit() {
         memset(&cfg, 0, sizeof(cfg));
         cfg.gridDim = dim3(16);
         cfg.blockDim = dim3(ROW_THREADS);
-        cfg.dynamicSmemBytes = ROW_PAGES * 4;
+        cfg.dynamicSmemBytes = row_smem(128, ROW_PAGES);
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 16;
@@ -258,7 +258,7 @@ static bool clusters_of_sixteen_fit() {
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
-        const bool fits = allow_smem(select_row_kernel<BF16, 128, 16>, ROW_PAGES * 4, true) == cudaSuccess &&
+        const bool fits = allow_smem(select_row_kernel<BF16, 128, 16>, row_smem(128, ROW_PAGES), true) == cudaSuccess &&
                           cudaOccupancyMaxActiveClusters(&n, select_row_kernel<BF16, 128, 16>, &cfg) == cudaSuccess && n > 0;
         if (!fits) cudaGetLastError();
         known[dev] = fits ? 2 : 1;
@@ -274,7 +274,7 @@ static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t
         const long long rows = (long long)tokens * p.c.kv_heads;
         int cl = 1;
         const int widest = clusters_of_sixteen_fit<BF16>() ? 16 : 8;
-        while (cl < widest && rows * cl * 2 <= 4ll * num_sms() && p.c.width >= 128 * cl) cl *= 2;
+        while (cl < widest && rows * cl * 2 <= 3ll * num_sms() && p.c.width >= 128 * cl) cl *= 2;
         return p.c.dim > 64 ? launch_select_cl<BF16, 128>(cl, p, tokens, stream) : launch_select_cl<BF16, 64>(cl, p, tokens, stream);
     }
     static bool done[64] = {false};
