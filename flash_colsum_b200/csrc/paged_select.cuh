@@ -72,15 +72,22 @@ struct Row {
     }
 };
 
-// Order-preserving keys: larger value, larger key; NaN is +inf, zeros are equal.  No value has key 0.
+// Order-preserving keys: larger value, larger key; zeros are equal.  No value has key 0 or one above +inf's.  (A score that is NaN
+// counts as +inf where it is summed in 64 bits -- as it is, since no error bound of its row is finite.)
 __device__ __forceinline__ uint32_t key_of(float s) {
-    const uint32_t bits = __float_as_uint(s != s ? INFINITY : s == 0.f ? 0.f : s);
-    return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    const int bits = __float_as_int(s + 0.f);
+    return min((uint32_t)(bits ^ (bits >> 31 | (int)0x80000000)), 0xff800000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ unsigned long long key_of(double s) {
     const unsigned long long bits = (unsigned long long)__double_as_longlong(s != s ? (double)INFINITY : s == 0.0 ? 0.0 : s);
     return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
+}
+
+__device__ __forceinline__ float log2_near(float x) {      // for guesses
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // E of a row whose parts sum up to `size` in magnitude and are at most `most`, over pages whose bounds reach up to `reach`; the
@@ -163,14 +170,14 @@ struct CloseList {
 // (`scores` has places for a multiple of four pages)
 template <int E>
 __device__ __forceinline__ void load_keys(const Row& r, const float* scores, int first, uint32_t (&keys)[E]) {
+    const uint32_t skip = (uint32_t)(r.lo - first), some = (uint32_t)(r.hi - r.lo);
 #pragma unroll
     for (int j = 0; j < E; j += 4) {
-        const int i = first + j;
-        const float4 q = i < r.pages ? *reinterpret_cast<const float4*>(scores + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        keys[j] = i >= r.lo && i < r.hi ? key_of(q.x) : 0u;
-        keys[j + 1] = i + 1 >= r.lo && i + 1 < r.hi ? key_of(q.y) : 0u;
-        keys[j + 2] = i + 2 >= r.lo && i + 2 < r.hi ? key_of(q.z) : 0u;
-        keys[j + 3] = i + 3 >= r.lo && i + 3 < r.hi ? key_of(q.w) : 0u;
+        const float4 q = first + j < r.pages ? *reinterpret_cast<const float4*>(scores + first + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        keys[j] = j - skip < some ? key_of(q.x) : 0u;
+        keys[j + 1] = j + 1 - skip < some ? key_of(q.y) : 0u;
+        keys[j + 2] = j + 2 - skip < some ? key_of(q.z) : 0u;
+        keys[j + 3] = j + 3 - skip < some ? key_of(q.w) : 0u;
     }
 }
 
@@ -353,8 +360,8 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
             else high = m0, at_high = n[0];
         };
         while (known && high - low > 1 && at_low - at_high > 24) {
-            const float top = __log2f((float)at_low + 0.5f), bottom = __log2f((float)at_high + 0.5f);
-            const float f = (top - __log2f((float)r.need + 0.5f)) / (top - bottom), d = (float)(high - low);
+            const float top = log2_near((float)at_low + 0.5f), bottom = log2_near((float)at_high + 0.5f);
+            const float f = __fdividef(top - log2_near((float)r.need + 0.5f), top - bottom), d = (float)(high - low);
             const uint32_t last = high - low - 1;
             auto guess = [&](float part) { return low + max(1u, min(last, (uint32_t)(part * d))); };
             narrow(guess(0.5f * f), guess(f), guess(0.5f + 0.5f * f));
