@@ -27,15 +27,25 @@ __device__ __forceinline__ void report(const Batch& c, int code) {
     if (c.status) atomicCAS(c.status, 0, code);
 }
 
-// Sequence of row `t`, for all threads of the block at once; `sequences` for a row behind the last one.
+// How many of 0 .. n - 1 come before the first for which `before` is false, by a converged warp: 32 of them looked at at a time.
+template <typename F>
+__device__ __forceinline__ int count_before(int n, F before) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 31) / 32;
+        const long long first = lo + (long long)lane * step;
+        const int whole = __popc(__ballot_sync(0xffffffffu, first < hi && before((int)min(first + step, (long long)hi) - 1)));
+        lo = min(hi, lo + whole * step);
+        if (lo < hi) hi = min(hi, lo + step) - 1;     // (the last of the next ones is not)
+    }
+    return lo;
+}
+
+// Sequence of row `t`, by a converged warp; `sequences` for a row behind the last one.
 __device__ __forceinline__ int sequence_of(const Batch& c, int t) {
     if (!c.starts) return t;
-    int n = 0;
-    for (int base = 0; base < c.sequences; base += blockDim.x) {
-        const int b = base + (int)threadIdx.x;
-        n += __syncthreads_count(b < c.sequences && c.starts[b + 1] <= t);
-    }
-    return n;
+    return count_before(c.sequences, [&](int i) { return c.starts[i + 1] <= t; });
 }
 
 // Position of row `t` of sequence `b` (negative where lens[b] counts fewer tokens than the sequence has rows).

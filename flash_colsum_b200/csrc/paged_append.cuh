@@ -143,12 +143,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 8) append_kernel(const __grid_
     int b = segment;
     long long j = 0, s0 = b, n = 1;
     if (c.starts) {
-        int seen = 0;
-        for (int base = 0; base < c.sequences; base += APPEND_THREADS) {
-            const int i = base + (int)threadIdx.x + 1;
-            seen += __syncthreads_count(i <= c.sequences && (c.starts[i] >> c.page_shift) + 2ll * i <= segment);
-        }
-        b = seen;
+        b = count_before(c.sequences, [&](int i) { return (c.starts[i + 1] >> c.page_shift) + 2ll * (i + 1) <= segment; });
         s0 = c.starts[b];
         j = (long long)segment - ((s0 >> c.page_shift) + 2ll * b);
         if (b == c.sequences) {     // no sequence: rows behind the last one

@@ -472,8 +472,7 @@ struct SharedLayout {
     static constexpr int bytes(int pages) { return OFF_SETS + 4 * pages + 1024; }
 };
 
-// grid: (CL * token tiles, kv heads); sequence b has the tiles from starts[b] / tile + b on, the last is for rows behind the last
-// sequence
+// grid: (CL * token tiles, kv heads); sequence b has the tiles from starts[b] / tile + b on, at least as many as it needs
 template <int DP, int STAGES, bool BF16, int CL>
 __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
     attend_shared_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
@@ -506,15 +505,13 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
     grid_launch_dependents();
 
     const int rank = (int)(blockIdx.x % CL), tile = (int)(blockIdx.x / CL), h = blockIdx.y, G = p.group;
-    int b = 0;
-    for (int base = 0; base < c.sequences; base += SHARED_THREADS) {
-        const int i = base + tid + 1;
-        b += __syncthreads_count(i <= c.sequences && c.starts[i] / p.tile_tokens + (long long)i <= tile);
-    }
+    const int b = count_before(c.sequences, [&](int i) { return c.starts[i + 1] / p.tile_tokens + (long long)(i + 1) <= tile; });
     const long long s0 = c.starts[b];
     if (b >= c.sequences) {        // (all CTAs of a cluster alike)
-        if (tile != (int)(gridDim.x / CL) - 1 || rank > 0) return;
-        for (long long t = max(s0, 0ll); t < c.tokens; ++t) {
+        // the tiles that no sequence needs share the rows behind the last one
+        const long long rest = tile - (s0 / p.tile_tokens + b), step = gridDim.x / CL - tile + rest;
+        if (rank > 0) return;
+        for (long long t = max(s0, 0ll) + rest; t < c.tokens; t += step) {
             if (p.fill_tail & 1)
                 for (int i = tid; i < G * c.dim; i += SHARED_THREADS)
                     p.out[t * p.out_st[0] + ((long long)h * G + i / c.dim) * p.out_st[1] + i % c.dim] = 0;

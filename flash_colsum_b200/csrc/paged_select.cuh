@@ -731,7 +731,7 @@ inline int tiles_row_bytes(int dim) { return 4 * dim + 16; }     // of a row of 
 inline int tiles_smem(int dim) { return 3 * 64 * tiles_row_bytes(dim); }
 
 // 64 tokens of one sequence, a share of the pages that they see.  grid: (token tiles, kv heads, splits); sequence b has the
-// tiles from starts[b] / 64 + b on, at least as many as it needs.
+// tiles from starts[b] / 64 + b on, at least as many as it needs (without starts, tile b alone).
 template <bool BF16>
 __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid_constant__ SelectParams p) {
     extern __shared__ __align__(16) uint8_t tiles_smem_raw[];
@@ -742,15 +742,18 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
     grid_launch_dependents();
     const Batch& c = p.c;
     const int D = c.dim, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long tile_id = (long long)blockIdx.x + max(0, p.t0 / TILE_TOKENS - 1);
-    int b = 0;
-    for (int base = 0; base < c.sequences; base += TILES_THREADS) {
-        const int i = base + tid + 1;
-        b += __syncthreads_count(i <= c.sequences && (c.starts[i] / TILE_TOKENS) + (long long)i <= tile_id);
+    int b;
+    long long s0, s1, first;
+    if (c.starts) {
+        const long long tile_id = (long long)blockIdx.x + max(0, p.t0 / TILE_TOKENS - 1);
+        b = count_before(c.sequences, [&](int i) { return c.starts[i + 1] / TILE_TOKENS + (long long)(i + 1) <= tile_id; });
+        if (b >= c.sequences) return;
+        s0 = c.starts[b], s1 = c.starts[b + 1];
+        first = s0 + (tile_id - (s0 / TILE_TOKENS + b)) * TILE_TOKENS;
+    } else {
+        b = p.t0 + (int)blockIdx.x;
+        s0 = first = b, s1 = b + 1;
     }
-    if (b >= c.sequences) return;
-    const long long s0 = c.starts[b], s1 = c.starts[b + 1];
-    const long long first = s0 + (tile_id - (s0 / TILE_TOKENS + b)) * TILE_TOKENS;
     if (s0 < 0 || s1 > c.tokens || first < s0 || first >= s1) return;
     if (first >= p.t1 || first + TILE_TOKENS <= p.t0) return;
     const int tokens = (int)min((long long)TILE_TOKENS, s1 - first), t_first = (int)first;
@@ -907,14 +910,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_con
     const long long at = row / c.kv_heads;
     const int h = (int)(row % c.kv_heads), t = p.t0 + (int)at;
     if (at >= p.t1 - p.t0) return;
-    int b = 0;
-    if constexpr (E > 0) {
-        const int lane = threadIdx.x & 31;
-        for (int base = 0; base < c.sequences; base += 32)
-            b += __popc(__ballot_sync(0xffffffffu, base + lane < c.sequences && c.starts[base + lane + 1] <= t));
-    } else {
-        b = sequence_of(c, t);
-    }
+    const int b = sequence_of(c, t);
     Row r = {};
     if (b < c.sequences) r.set(p, t, h, b, position_of(c, b, t));
     int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;

@@ -36,6 +36,7 @@ static int check_cache(const FcsPagedCache* c, Batch& out, int* status) {
     if (c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 || c->sequences <= 0 || c->table_width <= 0 || c->tokens <= 0)
         return fail(FCS_ERR_INVALID_ARGUMENT, "sizes must be positive (pages=%d kv_heads=%d sequences=%d table_width=%d tokens=%d)",
                     c->pages, c->kv_heads, c->sequences, c->table_width, c->tokens);
+    if (c->table_width > 1 << 28) return fail(FCS_ERR_UNSUPPORTED, "the table has too many pages a sequence (%d)", c->table_width);
     if (!c->page_table || !c->lens) return fail(FCS_ERR_INVALID_ARGUMENT, "page_table and lens must not be NULL");
     if (c->table_stride < c->table_width && c->sequences > 1)
         return fail(FCS_ERR_INVALID_ARGUMENT, "table_stride (%lld) is smaller than the table's width", (long long)c->table_stride);
@@ -190,9 +191,10 @@ constexpr int ROW_PAGES = 32768;       // scores that a CTA's shared memory hold
 
 // Scores of a row, with a place behind the last.
 static long long select_pitch(const FcsPagedCache* c) { return (c->table_width + 4ll) & ~3ll; }
-// Many tokens a sequence: the scores of 64 tokens and 64 pages are worth a tile of their own from about eight on.
+// Many tokens a sequence: the scores of 64 tokens and 64 pages are worth a tile of their own from about eight on.  And rows that
+// shared memory does not hold.
 static bool select_by_tiles(const FcsPagedCache* c) {
-    return c->starts && (c->tokens >= 8ll * c->sequences || select_pitch(c) > ROW_PAGES);
+    return (c->starts && c->tokens >= 8ll * c->sequences) || select_pitch(c) > ROW_PAGES;
 }
 
 struct SelectPlan {
@@ -281,7 +283,7 @@ static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t
     cudaError_t e = once_per_device(done, [] { return allow_smem(score_tiles_kernel<BF16>, tiles_smem(128)); });
     if (e != cudaSuccess) return e;
     const int first = p.t0 / TILE_TOKENS - 1 > 0 ? p.t0 / TILE_TOKENS - 1 : 0;
-    const dim3 grid((unsigned)((p.t1 - 1) / TILE_TOKENS - first + 1 + p.c.sequences), p.c.kv_heads, p.splits);
+    const dim3 grid(p.c.starts ? (unsigned)((p.t1 - 1) / TILE_TOKENS - first + 1 + p.c.sequences) : tokens, p.c.kv_heads, p.splits);
     e = launch(score_tiles_kernel<BF16>, grid, TILES_THREADS, tiles_smem(p.c.dim), 1, stream, p);
     if (e != cudaSuccess) return e;
     const long long rows = (long long)tokens * p.c.kv_heads;
@@ -306,8 +308,6 @@ static int select(const FcsPagedCache* cache, const void* query, const int64_t* 
     if (k < 1 || first < 0 || last < 1 || (long long)first + last > k)
         return fail(FCS_ERR_INVALID_ARGUMENT, "k must hold the first and the last pages (k=%d first=%d last=%d)", k, first, last);
     const SelectPlan plan = select_plan(cache);
-    if (!plan.tiles && plan.pitch > ROW_PAGES)
-        return fail(FCS_ERR_UNSUPPORTED, "one token a sequence chooses from at most %d pages, got %d", ROW_PAGES - 4, cache->table_width);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes)
         return fail(FCS_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes, got %zu", plan.bytes, workspace_bytes);
     p.query = static_cast<const uint16_t*>(query);

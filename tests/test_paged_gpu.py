@@ -270,6 +270,55 @@ def test_select_in_several_launches_under_a_wide_table():
     status_is(0)
 
 
+def test_one_token_a_sequence_under_a_table_that_shared_memory_does_not_hold():
+    a = Batch(16, [1] * 3, [16 * 70, 16 * 9, 5], 16, 2, 4, 64, FP16, packed=False, width=40000)
+    query = a.rows(4)
+    bounds = torch.stack([a.normal(a.N, 2, 64) - 1, a.normal(a.N, 2, 64) + 1], 2)
+    want = chosen_pages(query, bounds, 16, a.table, a.lens, None, 5, 1, 1)
+    assert torch.equal(select(a, query, bounds, 5, 1, 1).cpu(), want)
+    status_is(0)
+
+
+def test_many_short_sequences_and_a_long_rest():
+    """Sequences of none, one and some tokens in their thousands, and more rows behind them: every row finds its own."""
+    import flash_colsum_b200 as fc
+    g = torch.Generator().manual_seed(17)
+    new = [(7 * i) % 4 if i % 5 else 0 for i in range(2500)]
+    lens = [n + (i * 13) % 40 for i, n in enumerate(new)]
+    a = Batch(17, new, lens, 16, 1, 2, 16, BF16, tail=900)
+    owner = torch.full((a.T,), -1)
+    for t, b, pos in places(a.lens, a.starts, a.T):
+        owner[t] = b * 64 + pos
+    # values that say whose they are: value = (sequence, position), each exact in bf16 by its parts
+    value = torch.zeros(a.T, 1, 16, dtype=BF16)
+    part = torch.stack([(owner >> s) & 63 for s in (0, 6, 12)], 1).clamp(min=0)
+    value[:, 0, :3] = part.to(BF16)
+    key, query = a.rows(1) * 0, a.rows(2)
+    kp, vp = torch.zeros(a.N, 1, 16, 16, dtype=BF16).cuda(), torch.full((a.N, 1, 16, 16), 99.0, dtype=BF16).cuda()
+    bounds = torch.zeros(a.N, 1, 2, 16, dtype=BF16).cuda()
+    d = on_gpu(query, key, value, a.table, a.lens, a.starts)
+    out = fc.append_paged(d[1], d[2], kp, vp, d[3], d[4], starts=d[5], query=d[0], bounds=bounds)
+    assert torch.equal(out.cpu()[:a.T - 900], query[:a.T - 900]) and (out[a.T - 900:] == 0).all()
+    held = vp.cpu()
+    for t, b, pos in places(a.lens, a.starts, a.T):
+        assert torch.equal(held[int(a.table[b, pos // 16]), 0, pos % 16, :3], part[t].to(BF16))
+    pages = fc.select_pages(d[0], bounds, d[3], d[4], 3, page_size=16, starts=d[5])
+    last = torch.full((a.T,), -1)
+    for t, b, pos in places(a.lens, a.starts, a.T):
+        last[t] = pos // 16
+    assert torch.equal(pages.cpu()[:, 0].amax(1).long(), last)
+    own = torch.full((a.T, 1, 1), -1, dtype=torch.int32)
+    own[:, 0, 0] = last.int()
+    got = fc.attend_pages(d[0], kp, vp, d[3], d[4], own.cuda(), starts=d[5]).cpu().double()
+    # keys are zeros, so a result is the mean of what the token sees of its page
+    for t, b, pos in places(a.lens, a.starts, a.T):
+        seen = held[int(a.table[b, pos // 16]), 0, :pos % 16 + 1].double()
+        mean, spread = seen.mean(0), seen.abs().mean(0)
+        assert ((got[t] - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -14 * spread).all()
+    assert (got[a.T - 900:] == 0).all()
+    status_is(0)
+
+
 @pytest.mark.parametrize("more", [0, 20])
 def test_select_with_infinities_nan_and_pages_that_the_table_lacks(more):
     a = Batch(4, [3 + more, 1 + more], [16 * 60, 16 * 30], 16, 2, 2, 64, BF16)
