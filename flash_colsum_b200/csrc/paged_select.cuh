@@ -137,24 +137,41 @@ struct ExactScores {
             }
         }
     }
-    __device__ double operator()(const SelectParams& p, const Row& r, int i) const {
+    // Up to N pages at a time (page < 0: none), whose loads are in flight together.
+    template <int N>
+    __device__ void operator()(const SelectParams& p, const Row& r, const int (&page)[N], double (&score)[N]) const {
         const Batch& c = p.c;
-        const int lane = threadIdx.x & 31, page = physical_page(c, r.b, i);
-        if (page < 0) return -INFINITY;
-        double score = 0.0;
-        if (lane < c.dim / 4) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p.bounds + ((long long)page * c.kv_heads + r.h) * 2 * c.dim + lane * 8);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        const int lane = threadIdx.x & 31;
+        int at[N];
+        uint4 w[N];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 x = widen_pair<BF16>(words[e]);
-                score += part[2 * e] * (double)x.x;
-                score += part[2 * e + 1] * (double)x.y;
-            }
+        for (int i = 0; i < N; ++i) at[i] = page[i] >= 0 ? c.table[r.b * c.table_ld + page[i]] : -1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool there = at[i] >= 0 && at[i] < c.pages;
+            w[i] = there && lane < c.dim / 4 ? *reinterpret_cast<const uint4*>(p.bounds + ((long long)at[i] * c.kv_heads + r.h) * 2 * c.dim + lane * 8)
+                                             : make_uint4(0, 0, 0, 0);
+            if (!there) at[i] = -1;
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) score += __shfl_xor_sync(0xffffffffu, score, o);
-        return score;
+        for (int i = 0; i < N; ++i) {
+            const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            score[i] = 0.0;
+            if (lane < c.dim / 4)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = widen_pair<BF16>(words[e]);
+                    score[i] += part[2 * e] * (double)x.x;
+                    score[i] += part[2 * e + 1] * (double)x.y;
+                }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) score[i] += __shfl_xor_sync(0xffffffffu, score[i], o);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at[i] < 0) score[i] = -INFINITY;      // (said in the status word by whoever summed in 32 bits)
     }
 };
 
@@ -410,12 +427,20 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
                 const int warp = Team::SIZE > 32 ? threadIdx.x >> 5 : 0;
                 team.sync();               // (the keys have been read)
                 uint32_t todo = near;
-                for (int i = 0; todo; ++i, todo &= todo - 1)
-                    if (i % (Team::SIZE / 32) == warp) {
-                        const int at = __ffs(todo) - 1;
-                        const double s = score(p, r, team.close->page[at]);
-                        if (lane == 0) team.close->key[at] = key_of(s);
+                for (int i = 0; todo; ++i) {      // two at a time
+                    int at[2], page[2];
+                    double s[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        at[j] = __ffs(todo) - 1;
+                        todo &= todo - 1;
+                        page[j] = at[j] >= 0 ? team.close->page[at[j]] : -1;
                     }
+                    if (i % (Team::SIZE / 32) != warp) continue;
+                    score(p, r, page, s);
+                    if (lane == 0) team.close->key[at[0]] = key_of(s[0]);
+                    if (lane == 1 && at[1] >= 0) team.close->key[at[1]] = key_of(s[1]);
+                }
                 team.sync();
                 const unsigned long long mine = team.close->key[lane < m ? lane : 0];
                 ahead = 0;
@@ -443,11 +468,19 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
                 for (int j = 0; j < E; ++j) {
                     uint32_t todo = __ballot_sync(0xffffffffu, keys[j] >= low && keys[j] < high);
                     while (todo) {
-                        const int src = __ffs(todo) - 1;
-                        todo &= todo - 1;
-                        const int page = __shfl_sync(0xffffffffu, i, src) + j;
-                        const double s = score(p, r, page);
-                        if (lane == src) exact[page] = s;
+                        int src[4], page[4];
+                        double s[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            src[q] = __ffs(todo) - 1;
+                            todo &= todo - 1;
+                            page[q] = __shfl_sync(0xffffffffu, i, max(src[q], 0)) + j;
+                            if (src[q] < 0) page[q] = -1;
+                        }
+                        score(p, r, page, s);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (lane == src[q]) exact[page[q]] = s[q];
                     }
                 }
             });
@@ -897,7 +930,7 @@ constexpr int CHOOSE_THREADS = 128;
 
 // A warp per row, of at most 32 E pages, or (E = 0) a block.
 template <bool BF16, int E>
-__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(CHOOSE_THREADS, E == 16 ? 5 : 3) choose_kernel(const __grid_constant__ SelectParams p) {
     constexpr int ROWS = E > 0 ? CHOOSE_THREADS / 32 : 1;
     typedef BlockTeam<CHOOSE_THREADS, 16> Block;
     typedef WarpTeam<(E > 0 ? E : 4)> Warp;

@@ -163,14 +163,14 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
     p.q_heads = with_query ? r->q_heads : 0;
     p.fill_tail = r->fill_tail != 0;
     // A CTA has about 32 rows at a time, the heads of a group times the tokens of a page.  Of long calls it has more of the values
-    // and queries, whose heads share a token's rotation: 16384 tokens, 32 and 8 heads 121 us with one step, 89 with two, 85 with
-    // four, 89 with eight.
+    // and queries, whose heads share a token's rotation: 16384 tokens, 32 and 8 heads 121 us with one step, 78 with two, 76 with
+    // four; 1861 tokens of 7 sequences, 16 and 16 heads, pages of 16 13.2 us with one, 11.2 with two, 12.0 with four.
     const long long B = cache->sequences, T = cache->tokens, P = cache->page_size;
     const long long each = cache->starts ? (T / B < P ? (T + B - 1) / B : P) : 1;
     while (p.heads_shift < 3 && (each << p.heads_shift) < 32) ++p.heads_shift;
     const int heads = 1 << p.heads_shift;
     const long long ctas = T / each * (p.q_heads + cache->kv_heads) / heads;
-    p.steps = ctas >= 16ll * num_sms() ? 4 : 1;
+    p.steps = ctas >= 32ll * num_sms() ? 4 : ctas >= 8ll * num_sms() ? 2 : 1;
     p.key_groups = (cache->kv_heads + heads - 1) / heads;
     p.value_groups = (cache->kv_heads + heads * p.steps - 1) / (heads * p.steps);
     const long long segments = cache->starts ? T / P + 2 * B + 1 : B;
