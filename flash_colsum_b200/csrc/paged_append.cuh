@@ -10,6 +10,10 @@
 // (keys, values or queries), so that a page's bounds have one writer and need no atomics.  How many tokens the
 // sequences have is known on the device only: sequence b gets the CTAs from starts[b] / P + 2 b on, which is at least as many as it
 // has pages to write, and the ones it does not need leave at once.
+//
+// Memory bounds it, half of it reads and half writes: 16384 tokens, 32 query and 8 key/value heads of 128, bf16 (413 MB) 76 us,
+// 5.4 TB/s.  Short calls are chains of loads: starts, length, table and rows, 11 us for 1861 tokens in 7 sequences.  Blocks of
+// 128 threads, eight per SM: of 256 threads, four per SM, the long call took 98 us.
 #pragma once
 
 #include <cuda_bf16.h>

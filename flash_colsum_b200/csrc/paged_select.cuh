@@ -6,14 +6,19 @@
 //
 // Which of two pages is the better one must not hang on the order of a sum: pages are ordered by scores summed in 64 bits.  Few
 // need that.  Scores are summed in 32 bits first, which are off by at most
-//     E = c (sum |n| + sum |p|) max |bound|,
-// c counting the roundings; with t the k-th largest of them, a page above t + 2 E is chosen and one below t - 2 E is not whatever
+//     E = (c (sum |n| + sum |p|) + c' max(|n|, |p|)) max |bound|,
+// c and c' counting the roundings (score_error); with t the k-th largest of them, a page above t + 2 E is chosen and one below t - 2 E is not whatever
 // the exact scores are (the k-th largest of numbers each moved by E moves by E at most), and only the pages between are summed
 // again, in 64 bits.  Where E is not finite, all are.
 //
-// Two forms share that.  Few tokens a sequence (select_row_kernel): a cluster per row reads the bounds once, a warp
-// a page, and the first CTA chooses.  Many (score_tiles_kernel, choose_kernel): 64 tokens by 64 pages at a time on
-// tensor cores, n and p in two 16-bit parts each, and a warp or a block per row chooses from the scores.
+// Two forms share that.  Few tokens a sequence (select_row_kernel): a cluster per row reads the bounds once, and the first CTA
+// chooses.  Many (score_tiles_kernel, choose_kernel): 64 tokens by 64 pages at a time, n and p in two 16-bit pieces each, and a
+// warp or a block per row chooses from the scores.
+//
+// Measured, groups of four heads of 128, pages of 64: one query, 2048 pages (8.4 MB) 11 us, a chain of loads and barriers; 32
+// sequences x 256 to 512 pages (52 MB) 23 us, 13 of them while the bounds come at 4 TB/s, 5 of choosing behind them; 1021 tokens x
+// 512 pages 53 us, 27 of scores (matrix pipe 30 % busy) and 25 of choosing (2200 instructions a row, issue slots 64 % busy).
+// With 64-bit sums throughout these were 26, 42 and 1022 us.
 #pragma once
 
 #include <cuda_bf16.h>
