@@ -104,6 +104,33 @@ static cudaError_t once_per_device(bool (&done)[64], F set_up) {
     return e;
 }
 
+// Whether the current device can hold a cluster of sixteen CTAs of `kern` (asked once per device; `known` is the instance's: 0 not
+// asked, 1 no, 2 yes).
+template <typename F>
+static bool sixteen_fit(int (&known)[64], F* kern, int threads, int smem) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+    if (known[dev] == 0) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(16);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 16;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        const bool fits = allow_smem(kern, smem, true) == cudaSuccess &&
+                          cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0;
+        if (!fits) cudaGetLastError();
+        known[dev] = fits ? 2 : 1;
+    }
+    return known[dev] == 2;
+}
+
 // ------------------------------------------------------------------ append
 template <typename Ops>
 static cudaError_t launch_append(int rot, dim3 grid, cudaStream_t stream, const AppendParams& p) {
@@ -241,33 +268,6 @@ static cudaError_t launch_select_cl(int cl, const SelectParams& p, unsigned toke
                      : launch_select_row<BF16, DP, 1>(p, tokens, stream);
 }
 
-// Whether the current device can hold a cluster of sixteen CTAs of the row kernel (asked once per device).
-template <bool BF16>
-static bool clusters_of_sixteen_fit() {
-    static int known[64] = {0};         // 0: not asked, 1: no, 2: yes
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
-    if (known[dev] == 0) {
-        cudaLaunchConfig_t cfg;
-        memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3(16);
-        cfg.blockDim = dim3(ROW_THREADS);
-        cfg.dynamicSmemBytes = row_smem(128, ROW_PAGES);
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = 16;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        const bool fits = allow_smem(select_row_kernel<BF16, 128, 16>, row_smem(128, ROW_PAGES), true) == cudaSuccess &&
-                          cudaOccupancyMaxActiveClusters(&n, select_row_kernel<BF16, 128, 16>, &cfg) == cudaSuccess && n > 0;
-        if (!fits) cudaGetLastError();
-        known[dev] = fits ? 2 : 1;
-    }
-    return known[dev] == 2;
-}
-
 template <bool BF16>
 static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t stream) {
     const unsigned tokens = (unsigned)(p.t1 - p.t0);
@@ -275,7 +275,8 @@ static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t
         // CTAs of a row: as many as the device runs at once, 64 pages for each at least
         const long long rows = (long long)tokens * p.c.kv_heads;
         int cl = 1;
-        const int widest = clusters_of_sixteen_fit<BF16>() ? 16 : 8;
+        static int known[64] = {0};
+        const int widest = sixteen_fit(known, select_row_kernel<BF16, 128, 16>, ROW_THREADS, row_smem(128, ROW_PAGES)) ? 16 : 8;
         while (cl < widest && rows * cl * 2 <= 3ll * num_sms() && p.c.width >= 128 * cl) cl *= 2;
         return p.c.dim > 64 ? launch_select_cl<BF16, 128>(cl, p, tokens, stream) : launch_select_cl<BF16, 64>(cl, p, tokens, stream);
     }
@@ -341,14 +342,13 @@ static cudaError_t launch_attend(const CUtensorMap& km, const CUtensorMap& vm, c
     constexpr int STAGES = DP == 128 ? 3 : 4;
     using L = AttendLayout<DP, STAGES>;
     auto* kern = attend_kernel<DP, NT, STAGES, BF16, CL>;
-    static bool configured[64] = {false};
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev >= 64 || !configured[dev]) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+    if constexpr (CL == 16) {
+        static int known[64] = {0};
+        if (!sixteen_fit(known, kern, ATTEND_THREADS, L::BYTES)) return launch_attend<DP, NT, BF16, 8>(km, vm, p, stream);
+    } else {
+        static bool done[64] = {false};
+        const cudaError_t e = once_per_device(done, [&] { return allow_smem(kern, L::BYTES); });
         if (e != cudaSuccess) return e;
-        if (dev < 64) configured[dev] = true;
     }
     const dim3 grid((unsigned)((long long)CL * p.query_tiles * p.c.tokens), p.c.kv_heads);
     return launch(kern, grid, ATTEND_THREADS, L::BYTES, CL, stream, km, vm, p);
@@ -356,7 +356,8 @@ static cudaError_t launch_attend(const CUtensorMap& km, const CUtensorMap& vm, c
 
 template <int DP, int NT, bool BF16>
 static cudaError_t launch_attend_cl(int cl, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t s) {
-    return cl == 8   ? launch_attend<DP, NT, BF16, 8>(km, vm, p, s)
+    return cl == 16  ? launch_attend<DP, NT, BF16, 16>(km, vm, p, s)
+           : cl == 8 ? launch_attend<DP, NT, BF16, 8>(km, vm, p, s)
            : cl == 4 ? launch_attend<DP, NT, BF16, 4>(km, vm, p, s)
            : cl == 2 ? launch_attend<DP, NT, BF16, 2>(km, vm, p, s)
                      : launch_attend<DP, NT, BF16, 1>(km, vm, p, s);
@@ -376,7 +377,8 @@ static cudaError_t launch_shared(const CUtensorMap& km, const CUtensorMap& vm, c
 
 template <int DP, bool BF16>
 static cudaError_t launch_shared_cl(int cl, const CUtensorMap& km, const CUtensorMap& vm, const AttendParams& p, cudaStream_t s) {
-    return cl == 4   ? launch_shared<DP, BF16, 4>(km, vm, p, s)
+    return cl == 8   ? launch_shared<DP, BF16, 8>(km, vm, p, s)
+           : cl == 4 ? launch_shared<DP, BF16, 4>(km, vm, p, s)
            : cl == 2 ? launch_shared<DP, BF16, 2>(km, vm, p, s)
                      : launch_shared<DP, BF16, 1>(km, vm, p, s);
 }
@@ -445,8 +447,8 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     if (cache->starts && T >= 2 * B && p.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES) {
         // several tokens a sequence share what they chose in common
         const long long ctas = (T / p.tile_tokens > B ? T / p.tile_tokens : B) * cache->kv_heads;
-        const int cl = cluster_for(ctas, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 4);
-        if (4 * (T / p.tile_tokens + B + 1) > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
+        const int cl = cluster_for(ctas, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 8);
+        if (8 * (T / p.tile_tokens + B + 1) > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
         e = wide ? (bf16 ? launch_shared_cl<128, true>(cl, km, vm, p, stream) : launch_shared_cl<128, false>(cl, km, vm, p, stream))
                  : (bf16 ? launch_shared_cl<64, true>(cl, km, vm, p, stream) : launch_shared_cl<64, false>(cl, km, vm, p, stream));
         if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "attending failed to launch: %s", cudaGetErrorString(e));
@@ -456,7 +458,7 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     p.query_tiles = (p.group + 8 * nt - 1) / (8 * nt);
     const long long rows = T * cache->kv_heads * p.query_tiles;
     const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
-    const int cl = cluster_for(rows, 2, tiles >= 16 ? 8 : tiles >= 8 ? 4 : tiles >= 4 ? 2 : 1);     // (two tiles of keys for each CTA at least)
+    const int cl = cluster_for(rows, 2, tiles >= 32 ? 16 : tiles >= 16 ? 8 : tiles >= 8 ? 4 : tiles >= 4 ? 2 : 1);     // (two tiles of keys for each CTA at least)
     if (rows / cache->kv_heads * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
     if (wide)
         e = nt == 1 ? (bf16 ? launch_attend_cl<128, 1, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 1, false>(cl, km, vm, p, stream))

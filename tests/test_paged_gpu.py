@@ -362,6 +362,8 @@ ATTENDS = [
     ([65], [128 * 12 + 64], 128, 1, 32, 128, FP16, 7),
     ([40, 3], [900, 16 * 30 + 3], 16, 2, 10, 88, BF16, 20),
     ([100], [16 * 40], 16, 1, 1, 48, FP16, 11),
+    ([1], [64 * 130], 64, 1, 12, 96, BF16, 128),      # one row over sixteen CTAs, three tokens over eight
+    ([3], [64 * 130 + 7], 64, 1, 4, 128, FP16, 100),
 ]
 
 
