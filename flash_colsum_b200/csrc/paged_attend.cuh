@@ -16,7 +16,7 @@
 // few rows, are spread over the CTAs of a cluster, which join through distributed shared memory.
 //
 // Measured, groups of four heads of 128, bf16, pages of 64: 32 sequences x 32 pages (269 MB) 46 us, 5.9 TB/s; 4 sequences x 256
-// pages in clusters of eight 47 us; one sequence x 32 pages 7.8 us.  Three tiles of 32 KB in flight per CTA and two CTAs per SM;
+// pages in clusters of eight 47 us; one sequence x 32 pages in clusters of sixteen 7.6 us.  Three tiles of 32 KB in flight per CTA and two CTAs per SM;
 // with two tiles and three CTAs the 32 sequences take 53 us, with six tiles and one CTA 49 (and the four sequences 79).
 #pragma once
 

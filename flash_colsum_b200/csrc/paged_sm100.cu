@@ -444,10 +444,15 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     cudaError_t e;
     const long long T = cache->tokens, B = cache->sequences;
     p.tile_tokens = SHARED_COLS / p.group < 31 ? SHARED_COLS / p.group : 31;
-    if (cache->starts && T >= 2 * B && p.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES) {
-        // several tokens a sequence share what they chose in common
-        const long long ctas = (T / p.tile_tokens > B ? T / p.tile_tokens : B) * cache->kv_heads;
-        const int cl = cluster_for(ctas, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 8);
+    // Tokens of a sequence share what they chose in common, where there are enough of them: more than two a sequence, and blocks
+    // for all SMs or of eight tokens.  Measured, blocks against a token at a time, 32 pages of 64 for groups of four heads: 512
+    // blocks of two tokens 127 and 121 us; 256 of four 96 and 105, 192 of four 50 and 62; 128 of four 48 and 42 (58 and 52), 64
+    // of four 34 and 22; heads of their own, 64 of sixteen 53 and 60, 32 of sixteen 29 and 39.
+    const long long blocks = (p.tile_tokens > 0 && T / p.tile_tokens > B ? T / p.tile_tokens : B) * cache->kv_heads;
+    const long long together = T / B < p.tile_tokens ? T / B : p.tile_tokens;
+    if (cache->starts && T > 2 * B && p.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES &&
+        (blocks >= num_sms() || together >= 8)) {
+        const int cl = cluster_for(blocks, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 8);
         if (8 * (T / p.tile_tokens + B + 1) > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
         e = wide ? (bf16 ? launch_shared_cl<128, true>(cl, km, vm, p, stream) : launch_shared_cl<128, false>(cl, km, vm, p, stream))
                  : (bf16 ? launch_shared_cl<64, true>(cl, km, vm, p, stream) : launch_shared_cl<64, false>(cl, km, vm, p, stream));

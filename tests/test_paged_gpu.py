@@ -358,10 +358,16 @@ ATTENDS = [
     ([3], [32 * 200], 32, 2, 18, 72, FP16, 150),
     ([1], [64 * 300], 64, 1, 8, 128, FP16, 290),
     ([1] * 260, [1 + 2 * i for i in range(260)], 16, 1, 4, 16, BF16, 3),
+    # blocks of tokens: groups of four, eight, five and heads of their own, the last over one CTA, eight and four
+    ([70, 1, 0, 33], [1500, 40, 9, 128 * 5], 64, 8, 32, 128, BF16, 9),
+    ([40], [128 * 12 + 64], 128, 8, 64, 128, FP16, 7),
+    ([40, 3, 11], [900, 16 * 30 + 3, 77], 16, 10, 50, 88, BF16, 20),
+    ([300], [16 * 40], 16, 16, 16, 48, FP16, 11),
+    ([100], [16 * 40], 16, 1, 1, 48, FP16, 11),
+    ([100], [32 * 40 + 3], 32, 8, 8, 120, BF16, 13),
+    # tokens one by one
     ([70, 1, 0, 33], [1500, 40, 9, 128 * 5], 64, 2, 8, 128, BF16, 9),
     ([65], [128 * 12 + 64], 128, 1, 32, 128, FP16, 7),
-    ([40, 3], [900, 16 * 30 + 3], 16, 2, 10, 88, BF16, 20),
-    ([100], [16 * 40], 16, 1, 1, 48, FP16, 11),
     ([1], [64 * 130], 64, 1, 12, 96, BF16, 128),      # one row over sixteen CTAs, three tokens over eight
     ([3], [64 * 130 + 7], 64, 1, 4, 128, FP16, 100),
 ]
@@ -463,16 +469,19 @@ def test_attend_with_scores_at_the_ends_of_the_range():
         status_is(0)
 
 
-@pytest.mark.parametrize("D,P,group", [(128, 64, 4), (64, 16, 1), (96, 128, 8)])
-def test_attend_keeps_the_tokens_of_a_block_apart(D, P, group):
+# (one CTA a block, two and eight: blocks for all SMs, or of eight tokens and more)
+@pytest.mark.parametrize("D,P,group,H,tokens", [(128, 64, 4, 8, 90), (64, 16, 1, 2, 23), (96, 128, 8, 8, 41), (40, 32, 2, 20, 125),
+                                                (128, 16, 3, 16, 50)])
+def test_attend_keeps_the_tokens_of_a_block_apart(D, P, group, H, tokens):
     """Neighbouring tokens whose lists share pages: values that are not finite reach those that listed their page, and no others;
     nor do the keys behind a token, or a page that another token listed twice."""
     import flash_colsum_b200 as fc
-    a = Batch(21, [23], [P * 9 + 5], P, 2, 2 * group, D, BF16)
-    query, pools = a.rows(2 * group), [a.pool(), a.pool()]
-    pages = torch.full((a.T, 2, 6), -1, dtype=torch.int32)
+    held = -(-tokens // P) + 9
+    a = Batch(21, [tokens], [P * held + 5], P, H, H * group, D, BF16)
+    query, pools = a.rows(H * group), [a.pool(), a.pool()]
+    pages = torch.full((a.T, H, 6), -1, dtype=torch.int32)
     for t in range(a.T):
-        for h in range(2):
+        for h in range(H):
             order = torch.randperm(9, generator=a.g)[:5].int()
             pages[t, h, :5] = order
     for kind in ("nan in a page", "inf in keys and values", "nan in a later token", "twice"):
@@ -483,7 +492,8 @@ def test_attend_keeps_the_tokens_of_a_block_apart(D, P, group):
             v[int(a.table[0, 4]), 1, 0, :] = math.inf
             k[int(a.table[0, 5]), 0, 3, 1] = math.inf
         elif kind == "nan in a later token":          # the block's own page, which all of it lists
-            lists[:, :, 5] = 9 if P > 23 else lists[:, :, 5]
+            own = (torch.arange(a.T) + P * held + 5 - tokens) // P
+            lists[:, :, 5] = own[:, None].int()
             at = a.lens[0] - 2
             v[int(a.table[0, at // P]), :, int(at) % P, 0] = math.nan
         else:
@@ -507,8 +517,8 @@ def test_attend_keeps_the_tokens_of_a_block_apart(D, P, group):
 def test_attend_of_blocks_under_a_wide_table(width):
     """On both sides of the widest table that tokens share their pages under."""
     import flash_colsum_b200 as fc
-    a = Batch(22, [9, 30], [16 * 50, 16 * 70 + 1], 16, 2, 4, 64, FP16, width=width, tail=3)
-    query, pools = a.rows(4), [a.pool(), a.pool()]
+    a = Batch(22, [9, 30], [16 * 50, 16 * 70 + 1], 16, 2, 2, 64, FP16, width=width, tail=3)
+    query, pools = a.rows(2), [a.pool(), a.pool()]
     pages = listed_pages(a, 8)
     pages[2, 0, 0], pages[2, 1, 1] = 8192, 2 ** 31 - 1            # behind the token
     want, lse, spread, reach = attention(query, *pools, a.table, a.lens, a.starts, pages, 0.125)
