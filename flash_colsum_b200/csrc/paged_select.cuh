@@ -17,7 +17,7 @@
 //
 // Measured, groups of four heads of 128, pages of 64: one query, 2048 pages (8.4 MB) 11 us, a chain of loads and barriers; 32
 // sequences x 256 to 512 pages (52 MB) 23 us, 13 of them while the bounds come at 4 TB/s, 5 of choosing behind them; 1021 tokens x
-// 512 pages 53 us, 27 of scores (matrix pipe 30 % busy) and 25 of choosing (2200 instructions a row, issue slots 64 % busy).
+// 512 pages 54 us, 27 of scores (matrix pipe 30 % busy) and 27 of choosing (2100 instructions a row, issue slots 64 % busy).
 // With 64-bit sums throughout these were 26, 42 and 1022 us.
 #pragma once
 
@@ -563,8 +563,9 @@ __device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row&
 }
 
 // ------------------------------------------------------------------ few tokens a sequence
-constexpr int ROW_THREADS = 256;
-typedef BlockTeam<ROW_THREADS, 8> RowTeam;
+constexpr int ROW_THREADS = 128;
+constexpr int ROW_CTAS = 6;          // per SM (three of 256 threads: 32 sequences 23.4 us for 23.2)
+typedef BlockTeam<ROW_THREADS, 16> RowTeam;
 
 // grid: (CL * tokens, kv heads); shared memory: row_smem.  A warp takes 16 pages at a time, whose bounds bulk copies bring -- it
 // asks for the next 16 when it has read these -- as the rows of a matrix instruction: a lane reads eight neighbouring features,
@@ -574,7 +575,7 @@ __host__ __device__ constexpr int row_block_bytes(int dim) { return 16 * (4 * di
 inline int row_smem(int dim, int pitch) { return ROW_THREADS / 32 * row_block_bytes(dim) + 4 * pitch; }
 
 template <bool BF16, int DP, int CL>
-__global__ void __launch_bounds__(ROW_THREADS, 3) select_row_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const __grid_constant__ SelectParams p) {
     constexpr int CHUNKS = DP / 16;               // 32 of the 2 D features
     extern __shared__ __align__(16) uint8_t row_smem_raw[];
     __shared__ __align__(8) unsigned long long arrived[ROW_THREADS / 32];
@@ -602,32 +603,35 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) select_row_kernel(const __grid
     const int b = sequence_of(c, t);
     const long long pos = b < c.sequences ? position_of(c, b, t) : -1;
 
-    // a thread has one of the 2 D parts: the first D meet the lows, the others the highs
-    if (tid < 2 * DP) {
-        float part = 0.f;
-        if (tid < 2 * D && b < c.sequences) {
-            const bool low = tid < D;
-            const uint16_t* q = p.query + t * p.query_st[0] + (long long)h * p.group * p.query_st[1] + (low ? tid : tid - D);
+    // a thread has one or two of the 2 D parts: the first D meet the lows, the others the highs
+    {
+        float size = 0.f, most = 0.f;
+#pragma unroll
+        for (int i = tid; i < 2 * DP; i += ROW_THREADS) {
+            float part = 0.f;
+            if (i < 2 * D && b < c.sequences) {
+                const bool low = i < D;
+                const uint16_t* q = p.query + t * p.query_st[0] + (long long)h * p.group * p.query_st[1] + (low ? i : i - D);
 #pragma unroll 4
-            for (int g = 0; g < p.group; ++g) {
-                const float x = widen16<BF16>(q[g * p.query_st[1]]);
-                part += (low ? x < 0.f : !(x < 0.f)) ? x : 0.f;      // (NaN stays)
+                for (int g = 0; g < p.group; ++g) {
+                    const float x = widen16<BF16>(q[g * p.query_st[1]]);
+                    part += (low ? x < 0.f : !(x < 0.f)) ? x : 0.f;      // (NaN stays)
+                }
             }
+            float rest, rest2, z;
+            parts[0][i] = (uint16_t)round_pair<BF16>(part, 0.f, rest, z);
+            parts[1][i] = (uint16_t)round_pair<BF16>(rest, 0.f, rest2, z);
+            parts[2][i] = (uint16_t)round_pair<BF16>(rest2, 0.f, z, z);
+            parts[3][i] = 0;
+            size += fabsf(part);
+            most = max_or_nan(most, fabsf(part));
         }
-        float rest, rest2, z;
-        parts[0][tid] = (uint16_t)round_pair<BF16>(part, 0.f, rest, z);
-        parts[1][tid] = (uint16_t)round_pair<BF16>(rest, 0.f, rest2, z);
-        parts[2][tid] = (uint16_t)round_pair<BF16>(rest2, 0.f, z, z);
-        parts[3][tid] = 0;
-        float size = fabsf(part), most = size;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             size += __shfl_xor_sync(0xffffffffu, size, o);
             most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
         }
         if (lane == 0) warp_size[warp] = size, warp_most[warp] = most;
-    } else if (lane == 0) {
-        warp_size[warp] = warp_most[warp] = 0.f;
     }
     Row r = {};
     if (b < c.sequences) r.set(p, t, h, b, pos);

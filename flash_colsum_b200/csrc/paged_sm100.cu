@@ -277,7 +277,7 @@ static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t
         int cl = 1;
         static int known[64] = {0};
         const int widest = sixteen_fit(known, select_row_kernel<BF16, 128, 16>, ROW_THREADS, row_smem(128, ROW_PAGES)) ? 16 : 8;
-        while (cl < widest && rows * cl * 2 <= 3ll * num_sms() && p.c.width >= 128 * cl) cl *= 2;
+        while (cl < widest && rows * cl * 2 <= (long long)ROW_CTAS * num_sms() && p.c.width >= 128 * cl) cl *= 2;
         return p.c.dim > 64 ? launch_select_cl<BF16, 128>(cl, p, tokens, stream) : launch_select_cl<BF16, 64>(cl, p, tokens, stream);
     }
     static bool done[64] = {false};
