@@ -67,10 +67,12 @@ struct Row {
     int t, h, b;
     int pages, lo, hi;
     uint32_t need;
+    bool beyond;                // it sees pages that the table is too narrow for
     __device__ void set(const SelectParams& p, int t_, int h_, int b_, long long pos) {
         t = t_, h = h_, b = b_;
         const long long seen = pages_seen(p.c, pos);
         pages = (int)min(seen, (long long)p.c.width);
+        beyond = seen > pages;
         lo = min(p.first, pages);
         hi = (int)max((long long)lo, min((long long)pages, seen - p.last));
         need = (uint32_t)max(0, p.k - lo - (pages - hi));
@@ -550,6 +552,16 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
     for (int i = (int)place + team.rank(); i < p.k; i += Team::SIZE) out[i] = -1;
 }
 
+// Whether the table lacks a page of those that a row has without a score: its first `lo` ones, those from `hi` on and those past the
+// table's width.  A lane in `size`, each for its own.
+__device__ __forceinline__ bool lacks(const SelectParams& p, const Row& r, int lo, int hi, int rank, int size) {
+    const int* table = p.c.table + r.b * p.c.table_ld;
+    bool lacking = r.beyond;
+    for (int i = rank; i < lo; i += size) lacking |= (uint32_t)table[i] >= (uint32_t)p.c.pages;
+    for (int i = hi + rank; i < r.pages; i += size) lacking |= (uint32_t)table[i] >= (uint32_t)p.c.pages;
+    return lacking;
+}
+
 // The rows that need no scores: behind the last sequence, or with no more pages than are asked for.
 __device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row& r, int* out, int rank, int size) {
     if (b >= p.c.sequences) {
@@ -637,7 +649,10 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     if (b < c.sequences) r.set(p, t, h, b, pos);
     int* out = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
     if (b >= c.sequences || r.pages <= p.k) {       // (all CTAs of the cluster)
-        if (rank == 0) settled(p, b, r, out, tid, ROW_THREADS);
+        if (rank == 0) {
+            settled(p, b, r, out, tid, ROW_THREADS);
+            if (b < c.sequences && lacks(p, r, r.pages, r.pages, tid, ROW_THREADS)) report(c, FCS_STATUS_BAD_PAGE);
+        }
         if constexpr (CL > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         return;
     }
@@ -746,7 +761,10 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     }
     if constexpr (CL > 1) {
         cluster_sync();
-        if (rank > 0) return;
+        if (rank > 0) {       // (the last CTA has time to look up the pages that nobody scored)
+            if (rank == CL - 1 && lacks(p, r, r.lo, r.hi, tid, ROW_THREADS)) report(c, FCS_STATUS_BAD_PAGE);
+            return;
+        }
     } else {
         __syncthreads();
     }
@@ -763,6 +781,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     RowTeam team{row_scores, &close, room};
     const float error = score_error<BF16>(p, size, most, __uint_as_float(ends[2]), CHUNKS + 3, 3);
     choose<BF16>(p, r, team, ends, error, p.exact + ((long long)(t - p.t0) * c.kv_heads + h) * p.pitch, out);
+    if (CL == 1 && lacks(p, r, r.lo, r.hi, tid, ROW_THREADS)) report(c, FCS_STATUS_BAD_PAGE);
 }
 
 // ------------------------------------------------------------------ many tokens a sequence
@@ -877,6 +896,9 @@ __global__ void __launch_bounds__(TILES_THREADS) score_tiles_kernel(const __grid
         }
     };
     if (begin < end) fetch(begin);
+    // (the pages that none of these tokens lets compete are looked up here, by one of the splits; the others are by `fetch`)
+    if (blockIdx.z == 0)
+        for (long long i = pages + tid; i < seen && i <= c.width; i += TILES_THREADS) physical_page(c, b, i);
     for (int base = begin; base < end; base += TILE_PAGES) {
         __syncthreads();                // the tile before has been read
         if (my_vec == 0) missing[my_row] = next_page < 0;

@@ -1,0 +1,29 @@
+"""What the entry points over a paged cache do at their limits: pages that the table lacks, the largest lists, results in odd memory."""
+
+import pytest
+import torch
+
+from paged_reference import Batch, chosen_pages
+from test_paged_gpu import BF16, FP16, device_stays_sound, on_gpu, select, status_is  # noqa: F401  (the fixture is used by all)
+
+pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------- pages that the table lacks
+@pytest.mark.parametrize("tokens", [1, 3, 23, 90])     # a cluster a row, and tiles of 64 tokens
+@pytest.mark.parametrize("fault", ["narrow", "first", "own", "last but one", "competing", "behind", "other sequence's end"])
+@pytest.mark.parametrize("k", [8, 60])                # fewer than the pages that are seen, and all of them
+def test_a_selection_says_which_pages_it_misses(tokens, fault, k):
+    """Forced pages, and those of rows that take all they see, are looked up like those that compete."""
+    a = Batch(31, [tokens, 1], [16 * 50, 16 * 9], 16, 2, 2, 64, BF16, width=60)
+    query = a.rows(2)
+    bounds = torch.stack([a.normal(a.N, 2, 64) - 1, a.normal(a.N, 2, 64) + 1], 2)
+    if fault == "narrow":
+        a.table = a.table[:, :49].contiguous()       # the last token's page is the 50th
+    else:
+        sequence, entry = {"first": (0, 0), "own": (0, 49), "last but one": (0, 48), "competing": (0, 20), "behind": (0, 50),
+                           "other sequence's end": (1, 9)}[fault]
+        a.table[sequence, entry] = -1 if tokens % 2 else a.N
+    want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, k, 1, 2)
+    assert torch.equal(select(a, query, bounds, k, 1, 2).cpu(), want)
+    status_is(0 if fault in ("behind", "other sequence's end") else 5)
