@@ -549,7 +549,7 @@ __device__ void choose(const SelectParams& p, const Row& r, Team& team, uint32_t
             if (at < (uint32_t)p.k) out[at] = i + __ffs(taken) - 1;
         place += total;
     });
-    for (int i = (int)place + team.rank(); i < p.k; i += Team::SIZE) out[i] = -1;
+    for (uint32_t i = place + team.rank(); i < (uint32_t)p.k; i += Team::SIZE) out[i] = -1;
 }
 
 // Whether the table lacks a page of those that a row has without a score: its first `lo` ones, those from `hi` on and those past the
@@ -562,15 +562,16 @@ __device__ __forceinline__ bool lacks(const SelectParams& p, const Row& r, int l
     return lacking;
 }
 
-// The rows that need no scores: behind the last sequence, or with no more pages than are asked for.
+// The rows that need no scores: behind the last sequence, or with no more pages than are asked for.  (k may be the largest int: places
+// are counted without a sign, a step past it would have none.)
 __device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row& r, int* out, int rank, int size) {
     if (b >= p.c.sequences) {
         if (p.fill_tail)
-            for (int i = rank; i < p.k; i += size) out[i] = -1;
+            for (uint32_t i = rank; i < (uint32_t)p.k; i += size) out[i] = -1;
         return true;
     }
     if (r.pages > p.k) return false;
-    for (int i = rank; i < p.k; i += size) out[i] = i < r.pages ? i : -1;
+    for (uint32_t i = rank; i < (uint32_t)p.k; i += size) out[i] = i < (uint32_t)r.pages ? (int)i : -1;
     return true;
 }
 

@@ -27,3 +27,25 @@ def test_a_selection_says_which_pages_it_misses(tokens, fault, k):
     want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, k, 1, 2)
     assert torch.equal(select(a, query, bounds, k, 1, 2).cpu(), want)
     status_is(0 if fault in ("behind", "other sequence's end") else 5)
+
+
+# --------------------------------------------------------------------------- the largest lists
+@pytest.mark.parametrize("width", [4, 40000])         # a cluster a row, and tiles
+@pytest.mark.parametrize("k", [2 ** 31 - 1, 2 ** 31 - 128])
+def test_the_longest_list_ends_where_its_memory_ends(width, k):
+    """A list may be as long as its type counts: what steps through it leaves nothing in front of it or behind it."""
+    import flash_colsum_b200 as fc
+    a = Batch(32, [1], [16 * 3 + 1], 16, 1, 1, 16, BF16, packed=False, width=width)
+    query, table, lens = on_gpu(a.rows(1), a.table, a.lens)
+    bounds = torch.zeros(a.N, 1, 2, 16, dtype=BF16, device="cuda")
+    around = torch.full((k + 512,), 7, dtype=torch.int32, device="cuda")
+    out = around[256:256 + k].view(1, 1, k)
+    assert fc.select_pages(query, bounds, table, lens, k, page_size=16, out=out).data_ptr() == out.data_ptr()
+    assert out[0, 0, :4].tolist() == [0, 1, 2, 3]
+    assert int(out[0, 0, 4:].amin()) == int(out[0, 0, 4:].amax()) == -1
+    assert (around[:256] == 7).all() and (around[256 + k:] == 7).all()
+    del out, around
+    none = torch.zeros(2, dtype=torch.int32, device="cuda")       # a row behind the last sequence
+    out = fc.select_pages(query, bounds, table, lens, k, page_size=16, starts=none)
+    assert int(out.amin()) == int(out.amax()) == -1
+    status_is(0)
