@@ -423,6 +423,9 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     if ((rc = check_rows("value_pages", cache->value_pages, cache->value_stride, 3)) != FCS_OK) return rc;
     if ((rc = check_group(cache, q_heads)) != FCS_OK) return rc;
     if (!chosen || k < 1) return fail(FCS_ERR_INVALID_ARGUMENT, "chosen is NULL or has no entries (k=%d)", k);
+    // (the kernels count the entries of a block of up to sixteen tokens, and some steps past them, in an int)
+    static_assert((long long)SHARED_COLS * FCS_LIST_MAX <= 1 << 30, "the entries of a block");
+    if (k > FCS_LIST_MAX) return fail(FCS_ERR_UNSUPPORTED, "a list holds at most %d pages, got %d", FCS_LIST_MAX, k);
     if (scale != scale) return fail(FCS_ERR_INVALID_ARGUMENT, "scale is not a number");
     p.query = static_cast<const uint16_t*>(query);
     p.out = static_cast<uint16_t*>(out);

@@ -603,7 +603,7 @@ PyObject* py_attend_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!a.batch(query, THPVariable_Unpack(args[3]), THPVariable_Unpack(args[4]), starts)) Py_RETURN_NONE;
         if (!a.pools(query, THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2])) || !a.heads_ok(query)) Py_RETURN_NONE;
         if (!indices_ok(chosen, 3, a.dev) || chosen.size(0) != query.size(0) || chosen.size(1) != a.c.kv_heads ||
-            chosen.size(2) > 0x7fffffffLL / 256)
+            chosen.size(2) > FCS_LIST_MAX)
             Py_RETURN_NONE;
         int64_t st[2], out_st[2];
         if (given && (!like_rows(*given, query) || given->size(1) != query.size(1) || !rows_ready<2>(*given, out_st))) Py_RETURN_NONE;

@@ -37,6 +37,7 @@ from . import ops
 
 _TYPES = (torch.float16, torch.bfloat16)
 _PAGE_SIZES = (16, 32, 64, 128)
+_LIST_MAX = 1 << 26          # FCS_LIST_MAX
 
 
 def _rows_ready(t: torch.Tensor) -> bool:
@@ -290,7 +291,7 @@ def attend_pages(
         page_table, lens, starts: the batch (see the module).
         pages: (T, H_kv, k) int32, places in the sequence's row of the table, as :func:`select_pages` gives them
             but in any order; negative entries and pages behind the token's own weigh nothing, a page that is
-            listed twice weighs twice.
+            listed twice weighs twice.  At most 2 ** 26 of them.
         scale: score scale, default 1/sqrt(D).
         return_lse: return the natural logarithms of the sums of exp(score) too, for joining the result with
             that of other keys.
@@ -310,6 +311,8 @@ def attend_pages(
     _check_indices("pages", pages, query, 3)
     if tuple(pages.shape[:2]) != (query.shape[0], key_pages.shape[1]) or pages.shape[2] == 0:
         raise ValueError(f"pages must be ({query.shape[0]}, {key_pages.shape[1]}, k) with k >= 1, got {tuple(pages.shape)}")
+    if pages.shape[2] > _LIST_MAX:
+        raise ValueError(f"pages must have at most {_LIST_MAX} entries a list, got {pages.shape[2]}")
     if scale is not None and scale != scale:
         raise ValueError("scale is not a number")
     if out is not None:

@@ -407,8 +407,9 @@ int fcs_select_pages(const FcsPagedCache *cache, const void *query, const int64_
  * logarithm of the sum of exp(scale * score), or NULL.  chosen[tokens][kv_heads][k] in any order;
  * entries below 0 and pages behind the token's own weigh nothing, a page that is listed twice weighs
  * twice.  A query without a key gets zeros and an lse of -inf.  fill_tail is a sum: 1 for the rows of out behind the
- * last sequence, 2 for those of lse (-inf).
+ * last sequence, 2 for those of lse (-inf).  k is at most FCS_LIST_MAX.
  */
+#define FCS_LIST_MAX (1 << 26)
 int fcs_attend_pages(const FcsPagedCache *cache, const void *query, const int64_t *query_stride, int q_heads,
                      const int *chosen, int k, float scale, void *out, const int64_t *out_stride, float *lse,
                      int fill_tail, int *status, void *stream);

@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from paged_reference import Batch, chosen_pages
-from test_paged_gpu import BF16, FP16, device_stays_sound, on_gpu, select, status_is  # noqa: F401  (the fixture is used by all)
+from paged_reference import Batch, attention, chosen_pages
+from test_paged_gpu import BF16, FP16, attend_room, device_stays_sound, on_gpu, select, status_is  # noqa: F401  (a fixture of all)
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,24 @@ def test_the_longest_list_ends_where_its_memory_ends(width, k):
     out = fc.select_pages(query, bounds, table, lens, k, page_size=16, starts=none)
     assert int(out.amin()) == int(out.amax()) == -1
     status_is(0)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 9])         # sixteen CTAs a row, and a block of tokens
+def test_attention_over_the_longest_list(tokens):
+    """Entries from one end of the longest list to the other, nothing between them; one more entry is refused."""
+    import flash_colsum_b200 as fc
+    a = Batch(33, [tokens], [16 * 6], 16, 1, 1, 16, FP16)
+    query, pools = a.rows(1), [a.pool(), a.pool()]
+    pages = torch.full((a.T, 1, 2 ** 26), -1, dtype=torch.int32, device="cuda")
+    short = torch.full((a.T, 1, 5), -1, dtype=torch.int32)
+    for i, place in enumerate((0, 31, 2 ** 25 + 1, 2 ** 26 - 33, 2 ** 26 - 1)):
+        short[:, 0, i] = i
+        pages[:, :, place] = i
+    want, lse, spread, reach = attention(query, *pools, a.table, a.lens, a.starts, short, 0.25)
+    args = on_gpu(query, *pools, a.table, a.lens)
+    out, got = fc.attend_pages(*args, pages, starts=a.starts.cuda(), return_lse=True)
+    assert ((out.cpu().double() - want).abs() <= attend_room(FP16, 16, 80, want, spread, reach)).all()
+    assert ((got.cpu().double() - lse).abs() <= 24 * 2.0 ** -23 * reach + 2.0 ** -18 + lse.abs() * 2.0 ** -22).all()
+    status_is(0)
+    with pytest.raises(ValueError, match="at most 67108864 entries"):
+        fc.attend_pages(*args, pages[:, :, :1].expand(-1, -1, 2 ** 26 + 1), starts=a.starts.cuda())
