@@ -34,7 +34,7 @@ UNITS = {
         "colsum_single_pass.cuh", "select_topk.cuh", "colsum_fused_short.cuh", "host_api.h", "host_common.h") + [_ABI],
     _csrc("paged_sm100.cu")[0]: _csrc(
         "sm100_ptx.cuh", "paged.cuh", "paged_mma.cuh", "paged_append.cuh", "paged_select.cuh", "paged_attend.cuh",
-        "host_common.h") + [_ABI],
+        "host_api.h", "host_common.h") + [_ABI],
 }
 SOURCES = list(UNITS)
 HEADERS = sorted({header for headers in UNITS.values() for header in headers})

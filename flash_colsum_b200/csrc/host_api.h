@@ -58,3 +58,12 @@ int fcs_run_call(const FcsCall* call);
 // Copies in, computes, copies the result out; returns when the result is there.
 int fcs_run_host_call(const FcsHostCall* call);
 }
+
+// Whether the rows of a result, `dim` elements at these strides on two axes of `size` entries each, have no element in common, so
+// that each has one writer: the shorter stride holds a row, the longer one all rows of the shorter.  (The stride of an axis of one
+// entry says nothing.)
+inline bool fcs_rows_apart(const int64_t (&size)[2], const int64_t* stride, int64_t dim) {
+    if (size[0] <= 1 || size[1] <= 1) return (size[0] <= 1 || stride[0] >= dim) && (size[1] <= 1 || stride[1] >= dim);
+    const int inner = stride[1] <= stride[0] ? 1 : 0;
+    return stride[inner] >= dim && (stride[1 - inner] - dim) / stride[inner] >= size[inner] - 1;
+}

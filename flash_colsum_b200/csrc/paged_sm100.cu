@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include "../../include/flash_colsum_b200.h"
+#include "host_api.h"
 #include "host_common.h"
 #include "paged_append.cuh"
 #include "paged_attend.cuh"
@@ -23,6 +24,12 @@ static int check_rows(const char* name, const void* ptr, const int64_t* stride, 
         if (stride[i] < 0 || stride[i] % 8)
             return fail(FCS_ERR_INVALID_ARGUMENT, "%s strides must not be negative and be multiples of 8 elements", name);
     return FCS_OK;
+}
+
+static int check_result(const char* name, const FcsPagedCache* c, int q_heads, const int64_t* stride) {
+    const int64_t size[2] = {c->tokens, q_heads};
+    if (fcs_rows_apart(size, stride, c->dim)) return FCS_OK;
+    return fail(FCS_ERR_INVALID_ARGUMENT, "%s strides must keep its rows apart", name);
 }
 
 static int check_cache(const FcsPagedCache* c, Batch& out, int* status) {
@@ -154,6 +161,7 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
         if ((rc = check_rows("query", r->query, r->query_stride, 2)) != FCS_OK) return rc;
         if ((rc = check_rows("query_out", r->query_out, r->query_out_stride, 2)) != FCS_OK) return rc;
         if ((rc = check_group(cache, r->q_heads)) != FCS_OK) return rc;
+        if ((rc = check_result("query_out", cache, r->q_heads, r->query_out_stride)) != FCS_OK) return rc;
         if (r->q_heads > 65535 * 8) return fail(FCS_ERR_UNSUPPORTED, "too many query heads (%d)", r->q_heads);
     }
     if ((r->cos == nullptr) != (r->sin == nullptr)) return fail(FCS_ERR_INVALID_ARGUMENT, "cos and sin go together");
@@ -422,6 +430,7 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     if ((rc = check_rows("key_pages", cache->key_pages, cache->key_stride, 3)) != FCS_OK) return rc;
     if ((rc = check_rows("value_pages", cache->value_pages, cache->value_stride, 3)) != FCS_OK) return rc;
     if ((rc = check_group(cache, q_heads)) != FCS_OK) return rc;
+    if ((rc = check_result("out", cache, q_heads, out_stride)) != FCS_OK) return rc;
     if (!chosen || k < 1) return fail(FCS_ERR_INVALID_ARGUMENT, "chosen is NULL or has no entries (k=%d)", k);
     // (the kernels count the entries of a block of up to sixteen tokens, and some steps past them, in an int)
     static_assert((long long)SHARED_COLS * FCS_LIST_MAX <= 1 << 30, "the entries of a block");

@@ -378,6 +378,12 @@ bool rows_ready(const at::Tensor& t, int64_t (&st)[N]) {
     return (t.size(N) == 1 || t.stride(N) == 1) && any % 8 == 0 && (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0;
 }
 
+// A result of rows as the kernels write it.
+bool result_ready(const at::Tensor& t, int64_t (&st)[2]) {
+    const int64_t size[2] = {t.size(0), t.size(1)};
+    return rows_ready<2>(t, st) && fcs_rows_apart(size, st, t.size(2));
+}
+
 // A pool as the kernels take it: positive strides, no two entries in one place as far as the strides say.
 bool pool_ready(const at::Tensor& t, int64_t (&st)[3]) {
     if (!rows_ready<3>(t, st)) return false;
@@ -506,7 +512,7 @@ PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (query_in) {
             if (!like_rows(*query_in, key) || !a.heads_ok(*query_in)) Py_RETURN_NONE;
             if (query_out && (!like_rows(*query_out, key) || query_out->size(1) != query_in->size(1) ||
-                              !rows_ready<2>(*query_out, r.query_out_stride)))
+                              !result_ready(*query_out, r.query_out_stride)))
                 Py_RETURN_NONE;
             query = rows_ready<2>(*query_in, r.query_stride) ? *query_in : query_in->contiguous();
             rows_ready<2>(query, r.query_stride);
@@ -606,7 +612,7 @@ PyObject* py_attend_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
             chosen.size(2) > FCS_LIST_MAX)
             Py_RETURN_NONE;
         int64_t st[2], out_st[2];
-        if (given && (!like_rows(*given, query) || given->size(1) != query.size(1) || !rows_ready<2>(*given, out_st))) Py_RETURN_NONE;
+        if (given && (!like_rows(*given, query) || given->size(1) != query.size(1) || !result_ready(*given, out_st))) Py_RETURN_NONE;
         if (!rows_ready<2>(query, st)) query = query.contiguous();
         rows_ready<2>(query, st);
         pages = chosen.contiguous();

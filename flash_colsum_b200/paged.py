@@ -58,6 +58,15 @@ def _check_rows(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"head_dim must be a multiple of 8 from 8 to 128, got {t.shape[2]}")
 
 
+def _check_result(name: str, t: torch.Tensor) -> None:
+    """Memory for a result: rows that can be written in pieces of 16 bytes, none of which lies in another."""
+    rows = sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1)
+    apart = all(s >= t.shape[2] for s, _ in rows) and (len(rows) < 2 or rows[1][0] >= rows[0][0] * (rows[0][1] - 1) + t.shape[2])
+    if not _rows_ready(t) or not apart:
+        raise ValueError(f"{name} needs unit inner stride, other strides in multiples of 8 elements that keep its rows apart, and a "
+                         f"16-byte aligned base, got strides {t.stride()}")
+
+
 def _check_like(name: str, t: torch.Tensor, rows: torch.Tensor, shape) -> None:
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
@@ -151,7 +160,7 @@ def append_paged(
         interleaved: rotate feature 2 i with feature 2 i + 1 instead.
         bounds: (N, H_kv, 2, D) of the pools' type, contiguous: per page and head the smallest and the largest value of every
             feature, over the (rotated) keys written since the page's slot 0 was; kept up to date in place.
-        query_out: memory for the rotated queries; may be ``query``.
+        query_out: memory for the rotated queries, whose rows do not overlap; may be ``query``.
 
     Returns:
         The rotated queries (T, H_q, D), or None without ``query``.
@@ -196,8 +205,7 @@ def append_paged(
         _check_like("query", query, key, (key.shape[0], query.shape[1], D))
         if query_out is not None:
             _check_like("query_out", query_out, query, query.shape)
-            if not _rows_ready(query_out):
-                raise ValueError(f"query_out needs unit inner stride and other strides in multiples of 8 elements, got {query_out.stride()}")
+            _check_result("query_out", query_out)
     if key.shape[0] == 0:
         return query_out if query is None or query_out is not None else torch.empty_like(query, memory_format=torch.contiguous_format)
     out = _native(key.device).append_paged(key, value, key_pages, value_pages, page_table, lens, starts, query, cos, sin, positions,
@@ -295,7 +303,7 @@ def attend_pages(
         scale: score scale, default 1/sqrt(D).
         return_lse: return the natural logarithms of the sums of exp(score) too, for joining the result with
             that of other keys.
-        out: (T, H_q, D) of the pools' type, for the result.
+        out: (T, H_q, D) of the pools' type, for the result; its rows do not overlap.  May be ``query``.
 
     Returns:
         (T, H_q, D), and with ``return_lse`` (T, H_q) fp32.  A query that sees no key gets zeros and -inf.
@@ -317,8 +325,7 @@ def attend_pages(
         raise ValueError("scale is not a number")
     if out is not None:
         _check_like("out", out, query, query.shape)
-        if not _rows_ready(out):
-            raise ValueError(f"out needs unit inner stride and other strides in multiples of 8 elements, got {out.stride()}")
+        _check_result("out", out)
     if query.shape[0] == 0:
         res = out if out is not None else torch.empty_like(query, memory_format=torch.contiguous_format)
         return (res, torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)) if return_lse else res

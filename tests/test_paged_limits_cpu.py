@@ -3,10 +3,27 @@
 import pytest
 
 from flash_colsum_b200 import _cabi
-from test_paged_cpu import attend
+from test_paged_cpu import append, attend, cache, rows
 
 
 @pytest.mark.parametrize("k", [2 ** 26 + 1, 2 ** 27, 2 ** 31 - 1])
 def test_lists_that_the_attention_cannot_count_are_refused(k):
     assert attend(k=k) < 0
     assert "at most 67108864 pages" in _cabi.last_error()
+
+
+@pytest.mark.parametrize("stride", [(0, 128), (1024, 0), (0, 0), (1024, 120), (1016, 128), (128, 128), (128, 632), (8, 1024)])
+def test_results_whose_rows_overlap_are_refused(stride):
+    """Five tokens of eight heads of 128."""
+    assert append(r=rows(query_out_stride=stride)) < 0
+    assert "query_out strides must keep its rows apart" in _cabi.last_error()
+    assert attend(out_st=stride) < 0
+    assert "out strides must keep its rows apart" in _cabi.last_error()
+
+
+@pytest.mark.parametrize("tokens,heads,stride", [(5, 8, (1024, 128)), (5, 8, (128, 640)), (5, 8, (1024, 1 << 40)), (1, 8, (0, 128)), (5, 1, (128, 0)),
+                                                 (1, 1, (0, 0))])
+def test_results_whose_rows_do_not_are_checked_further(tokens, heads, stride):
+    c = cache(tokens=tokens, kv_heads=1)
+    assert attend(c, heads=heads, out_st=stride, k=0) < 0
+    assert "chosen" in _cabi.last_error()

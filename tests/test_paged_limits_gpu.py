@@ -70,3 +70,41 @@ def test_attention_over_the_longest_list(tokens):
     status_is(0)
     with pytest.raises(ValueError, match="at most 67108864 entries"):
         fc.attend_pages(*args, pages[:, :, :1].expand(-1, -1, 2 ** 26 + 1), starts=a.starts.cuda())
+
+
+# --------------------------------------------------------------------------- memory for results
+def test_results_in_memory_that_overlaps_are_refused():
+    import flash_colsum_b200 as fc
+    T, H, heads, D = 5, 2, 4, 64
+    a = Batch(34, [T], [40], 16, H, heads, D, BF16)
+    q, k, kp, vp, table, lens, starts = on_gpu(a.rows(heads), a.rows(H), a.pool(), a.pool(), a.table, a.lens, a.starts)
+    pages = torch.zeros(T, H, 1, dtype=torch.int32, device="cuda")
+    memory = torch.zeros(1 << 16, dtype=BF16, device="cuda")
+    for stride in ((0, D), (heads * D, 0), (0, 0), (heads * D, D - 8), (heads * D - 8, D), (D, D), (D, T * D - 8), (8, 4 * D)):
+        odd = memory.as_strided((T, heads, D), (*stride, 1))
+        with pytest.raises(ValueError, match="query_out needs .* keep its rows apart"):
+            fc.append_paged(k, k, kp, vp, table, lens, starts=starts, query=q, query_out=odd)
+        with pytest.raises(ValueError, match="out needs .* keep its rows apart"):
+            fc.attend_pages(q, kp, vp, table, lens, pages, starts=starts, out=odd)
+    assert (memory == 0).all()
+    status_is(0)
+
+
+def test_results_in_any_memory_that_does_not():
+    """Heads outside the tokens, gaps, one token or one head at any stride, and the queries' own memory."""
+    import flash_colsum_b200 as fc
+    for T, H, heads, D in ((5, 2, 4, 64), (1, 2, 4, 64), (40, 8, 8, 64), (5, 1, 1, 128), (1, 1, 1, 8)):
+        a = Batch(35, [T], [T + 70], 16, H, heads, D, BF16)
+        q, k, kp, vp, table, lens, starts = on_gpu(a.rows(heads), a.rows(H), a.pool(), a.pool(), a.table, a.lens, a.starts)
+        pages = torch.arange(3, dtype=torch.int32, device="cuda").expand(T, H, 3)
+        turn = torch.rand(T + 70, D // 2 // 8 * 8, device="cuda") if D >= 16 else None
+        call = dict(starts=starts, query=q, cos=turn, sin=turn)
+        turned = fc.append_paged(k, k, kp, vp, table, lens, **call)
+        want = fc.attend_pages(turned, kp, vp, table, lens, pages, starts=starts)
+        strides = [(D, T * D), (heads * D + 8, D), (heads * (D + 8), D + 8), (heads * D if T > 1 else 0, D if heads > 1 else 0)]
+        for stride in strides:
+            odd = torch.full((1 << 17,), 7.0, dtype=BF16, device="cuda").as_strided((T, heads, D), (*stride, 1))
+            assert fc.append_paged(k, k, kp, vp, table, lens, **call, query_out=odd).data_ptr() == odd.data_ptr()
+            assert torch.equal(odd, turned)
+            assert torch.equal(fc.attend_pages(odd, kp, vp, table, lens, pages, starts=starts, out=odd), want)
+    status_is(0)
