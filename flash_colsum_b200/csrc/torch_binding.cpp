@@ -392,6 +392,15 @@ bool pool_ready(const at::Tensor& t, int64_t (&st)[3]) {
     return true;
 }
 
+// Memory of the caller's that a call writes, asked for when nothing can refuse the call any more: a tensor that shares its memory until
+// it is written gets its own, and the version counter tells autograd that a saved tensor has changed.  (Tensors of inference mode
+// have none.)
+void* written(const at::Tensor& t) {
+    void* at = t.mutable_data_ptr();
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return at;
+}
+
 // The batch and, unless they are not given, the pools of a call; whatever had to be laid out anew is held until it returns.
 struct PagedArgs {
     FcsPagedCache c = {};
@@ -431,7 +440,7 @@ struct PagedArgs {
         if (n[0] < 1 || n[0] > 0x7fffffffLL || n[1] < 1 || n[1] > 65535 || n[3] != c.dim) return false;
         if (n[2] != 16 && n[2] != 32 && n[2] != 64 && n[2] != 128) return false;
         if (!pool_ready(k, c.key_stride) || !pool_ready(v, c.value_stride)) return false;
-        c.key_pages = const_cast<void*>(k.const_data_ptr());
+        c.key_pages = const_cast<void*>(k.const_data_ptr());      // (to be read; append_paged asks again)
         c.value_pages = const_cast<void*>(v.const_data_ptr());
         c.pages = (int)n[0];
         c.kv_heads = (int)n[1];
@@ -506,7 +515,6 @@ PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 bounds->size(3) != a.c.dim || bounds->scalar_type() != key.scalar_type() || bounds->device() != a.dev ||
                 !bounds->is_contiguous() || (reinterpret_cast<uintptr_t>(bounds->const_data_ptr()) & 15))
                 Py_RETURN_NONE;
-            r.bounds = const_cast<void*>(bounds->const_data_ptr());
         }
         if (query_out && !query_in) Py_RETURN_NONE;
         if (query_in) {
@@ -519,8 +527,8 @@ PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
             r.fill_tail = query_out == nullptr;
             out = query_out ? *query_out : empty_on(query.sizes(), query.scalar_type(), a.dev);
             rows_ready<2>(out, r.query_out_stride);
+            r.query_out = query_out ? written(out) : out.mutable_data_ptr();
             r.query = query.const_data_ptr();
-            r.query_out = out.mutable_data_ptr();
             r.q_heads = (int)query.size(1);
         }
         if (!rows_ready<2>(key, r.key_stride)) key = key.contiguous();
@@ -529,6 +537,9 @@ PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         rows_ready<2>(value, r.value_stride);
         r.key = key.const_data_ptr();
         r.value = value.const_data_ptr();
+        a.c.key_pages = written(THPVariable_Unpack(args[2]));
+        a.c.value_pages = written(THPVariable_Unpack(args[3]));
+        if (bounds) r.bounds = written(*bounds);
         WithoutGil nogil;
         rc = g_append_paged(&a.c, &r, a.status, a.stream());
     }
@@ -575,9 +586,10 @@ PyObject* py_select_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
         rows_ready<2>(query, st);
         const int64_t bytes[1] = {(int64_t)g_select_pages_workspace(&a.c)};
         const at::Tensor scratch = empty_on(c10::IntArrayRef(bytes, 1), at::kByte, a.dev);
+        int* const chosen = static_cast<int*>(given ? written(out) : out.mutable_data_ptr());
         WithoutGil nogil;
         rc = g_select_pages(&a.c, query.const_data_ptr(), st, (int)query.size(1), bounds.const_data_ptr(), k, first, last,
-                            static_cast<int*>(out.mutable_data_ptr()), given == nullptr, scratch.mutable_data_ptr(),
+                            chosen, given == nullptr, scratch.mutable_data_ptr(),
                             (size_t)bytes[0], a.status, a.stream());
     }
     if (rc != FCS_OK) return raise_library_error(rc);
@@ -619,9 +631,10 @@ PyObject* py_attend_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
         out = given ? *given : empty_on(query.sizes(), query.scalar_type(), a.dev);
         rows_ready<2>(out, out_st);
         if (with_lse) lse = empty_f32(query.size(0), query.size(1), a.dev);
+        void* const result = given ? written(out) : out.mutable_data_ptr();
         WithoutGil nogil;
         rc = g_attend_pages(&a.c, query.const_data_ptr(), st, (int)query.size(1), static_cast<const int*>(pages.const_data_ptr()),
-                            (int)pages.size(2), (float)scale, out.mutable_data_ptr(), out_st,
+                            (int)pages.size(2), (float)scale, result, out_st,
                             with_lse ? static_cast<float*>(lse.mutable_data_ptr()) : nullptr, given ? 2 : 3, a.status, a.stream());
     }
     if (rc != FCS_OK) return raise_library_error(rc);

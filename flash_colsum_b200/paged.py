@@ -19,8 +19,8 @@ stream order, so that a captured call follows them.
 
 The pools are (N, H_kv, P, D) fp16 or bf16 tensors, P 16, 32, 64 or 128 and D a multiple of 8 up to 128,
 with unit inner stride and any order of the others in multiples of 8 elements -- the two halves of one
-(N, 2, H_kv, P, D) tensor, or a (N, P, H_kv, D) one seen through ``transpose(1, 2)``.  They are written and read in place;
-there is no gradient.  A page that a token needs and the table does not have is neither written nor
+(N, 2, H_kv, P, D) tensor, or a (N, P, H_kv, D) one seen through ``transpose(1, 2)``.  They are written and read in place, and count
+as changed in place for autograd; there is no gradient.  A page that a token needs and the table does not have is neither written nor
 read, and :func:`device_status` says so (5); a position that the rotation's tables do not have, likewise (6).
 
 Calls run on the current stream of the tensors' device without synchronising.

@@ -108,3 +108,69 @@ def test_results_in_any_memory_that_does_not():
             assert torch.equal(odd, turned)
             assert torch.equal(fc.attend_pages(odd, kp, vp, table, lens, pages, starts=starts, out=odd), want)
     status_is(0)
+
+
+def a_step(seed):
+    a = Batch(seed, [3], [40], 16, 2, 4, 64, BF16)
+    q, k, v, kp, vp, table, lens, starts = on_gpu(a.rows(4), a.rows(2), a.rows(2), a.pool(), a.pool(), a.table, a.lens, a.starts)
+    return q, k, v, kp, vp, torch.stack([kp.amin(2), kp.amax(2)], 2), table, lens, starts
+
+
+def test_pools_that_share_their_memory_until_they_are_written():
+    """A lazy copy of pools, bounds and results gets memory of its own when it is written, and only then."""
+    import flash_colsum_b200 as fc
+    q, k, v, kp, vp, bounds, table, lens, starts = a_step(36)
+    first = [t.clone() for t in (kp, vp, bounds, q)]
+    own = [t.clone() for t in (kp, vp, bounds)]
+    want = fc.append_paged(k, v, own[0], own[1], table, lens, starts=starts, query=q, bounds=own[2])
+    pages = fc.select_pages(want, own[2], table, lens, 2, page_size=16, starts=starts)
+    out = fc.attend_pages(want, *own[:2], table, lens, pages, starts=starts)
+
+    lazy = [torch._lazy_clone(t) for t in (kp, vp, bounds, q)]
+    turned = fc.append_paged(k, v, lazy[0], lazy[1], table, lens, starts=starts, query=lazy[3], bounds=lazy[2], query_out=lazy[3])
+    assert turned.data_ptr() == lazy[3].data_ptr() and torch.equal(turned, want)
+    assert all(torch.equal(x, y) for x, y in zip(lazy, own))
+    assert all(torch.equal(x, y) for x, y in zip((kp, vp, bounds, q), first))
+
+    lazy = [torch._lazy_clone(t) for t in (*own, want, pages, out)]
+    assert torch.equal(fc.select_pages(lazy[3], lazy[2], table, lens, 2, page_size=16, starts=starts), pages)
+    assert torch.equal(fc.attend_pages(lazy[3], lazy[0], lazy[1], table, lens, lazy[4], starts=starts), out)
+    assert all(torch._C._is_cow_tensor(t) for t in lazy)          # (they have been read)
+    pages_out, attend_out = lazy[4], lazy[5]
+    fc.select_pages(want, own[2], table, lens, 2, page_size=16, starts=torch.tensor([0, 1], dtype=torch.int32).cuda(), out=pages_out)
+    fc.attend_pages(-want, *own[:2], table, lens, pages, starts=starts, out=attend_out)
+    again = fc.select_pages(want, own[2], table, lens, 2, page_size=16, starts=starts)
+    assert torch.equal(pages, again) and torch.equal(out, fc.attend_pages(want, *own[:2], table, lens, pages, starts=starts))
+    assert not torch.equal(attend_out, out)
+    # a call that is refused has not asked for memory
+    lazy = [torch._lazy_clone(t) for t in (kp, vp, bounds)]
+    with pytest.raises(ValueError):
+        fc.append_paged(k, v[:2], lazy[0], lazy[1], table, lens, starts=starts, bounds=lazy[2])
+    assert all(torch._C._is_cow_tensor(t) for t in lazy)
+    status_is(0)
+
+
+def test_autograd_sees_what_the_calls_write():
+    import flash_colsum_b200 as fc
+    q, k, v, kp, vp, bounds, table, lens, starts = a_step(37)
+    pages = torch.zeros(3, 2, 2, dtype=torch.int32, device="cuda")
+    out, turned = torch.zeros_like(q), torch.zeros_like(q)
+    calls = [((kp, vp, bounds, turned), lambda: fc.append_paged(k, v, kp, vp, table, lens, starts=starts, query=q, bounds=bounds, query_out=turned)),
+             ((pages,), lambda: fc.select_pages(q, bounds, table, lens, 2, page_size=16, starts=starts, out=pages)),
+             ((out,), lambda: fc.attend_pages(q, kp, vp, table, lens, pages, starts=starts, out=out))]
+    for changed, call in calls:
+        before = [t._version for t in changed]
+        others = [t for t in (q, k, v, kp, vp, bounds, pages, out, turned) if all(t is not c for c in changed)]
+        kept = [t._version for t in others]
+        call()
+        assert all(t._version > n for t, n in zip(changed, before)) and [t._version for t in others] == kept
+    weight = torch.ones_like(kp, requires_grad=True)
+    loss = (weight * kp).sum()
+    calls[0][1]()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        held = [t.clone() for t in (kp, vp, bounds)]
+    fc.append_paged(k, v, held[0], held[1], table, lens, starts=starts, bounds=held[2])      # (tensors without a counter)
+    assert torch.equal(held[0], kp) and torch.equal(held[2], bounds)
+    status_is(0)
