@@ -101,13 +101,13 @@ __device__ __forceinline__ float log2_near(float x) {      // for guesses
 // scores were formed by matrix instructions, 16 terms at a time from zero, of parts in `pieces` 16-bit pieces.  Of the whole's
 // magnitude: roundings of 2^-24, the group's sums and `adds` sums behind the matrix instructions, and what the pieces leave.  Of
 // the largest term: in each of D / 8 steps up to 2^-23 for 17 terms, where a tensor core drops what lies below its last bit.  And
-// half of fp16's smallest step of every part.  Sums that may overflow are no sums (NaN likewise), and products that underflow
+// half of fp16's smallest step of every part -- none of which may pass fp16's range, whatever they sum up to.  Sums that may overflow are no sums (NaN likewise), and products that underflow
 // lose what no share of the whole covers: 1e-36 is 85 times the smallest normal number.
 template <bool BF16>
 __device__ __forceinline__ float score_error(const SelectParams& p, float size, float most, float reach, int adds, int pieces) {
     const float left = BF16 ? (pieces == 2 ? 3.9e-6f : 0.f) : (pieces == 2 ? 2.4e-7f : 0.f);
     float error = ((float)(p.group + adds + 2) * 6.1e-8f + left) * size + (float)p.c.dim / 8.f * 17.f * 1.2e-7f * most;
-    if (!BF16) error = size < 6e4f ? error + 2.f * p.c.dim * 3e-8f : INFINITY;
+    if (!BF16) error = most < 6e4f ? error + 2.f * p.c.dim * 3e-8f : INFINITY;
     return size * reach < 1e37f ? error * reach + 1e-36f : INFINITY;
 }
 

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from paged_reference import Batch, attention, chosen_pages
+from paged_reference import Batch, attention, chosen_pages, places
 from test_paged_gpu import BF16, FP16, attend_room, device_stays_sound, on_gpu, select, status_is  # noqa: F401  (a fixture of all)
 
 pytestmark = pytest.mark.gpu
@@ -173,4 +173,39 @@ def test_autograd_sees_what_the_calls_write():
         held = [t.clone() for t in (kp, vp, bounds)]
     fc.append_paged(k, v, held[0], held[1], table, lens, starts=starts, bounds=held[2])      # (tensors without a counter)
     assert torch.equal(held[0], kp) and torch.equal(held[2], bounds)
+    status_is(0)
+
+
+# --------------------------------------------------------------------------- sums in 64 bits
+@pytest.mark.parametrize("tokens", [2, 20])           # a cluster a row, and tiles
+@pytest.mark.parametrize("group,D,size", [(32, 128, 20.0), (8, 128, 80.0), (4, 64, 1500.0), (1, 64, 2.0 ** 15)])
+def test_large_queries_of_half_precision_need_no_more_sums_than_others(tokens, group, D, size):
+    """Parts whose magnitudes sum up to more than fp16 holds, each of them within its range: the 64-bit sums that the workspace has
+    room for stay unwritten but for rows with many pages next to the border.  Parts past it: all are."""
+    from flash_colsum_b200 import _cabi, ops
+    import ctypes
+    pages, k = 500, 24
+    a = Batch(38, [tokens], [16 * pages], 16, 1, group, D, FP16)
+    query = a.rows(group)
+    query = (query * (size / (1.0 if group > 1 else 4.0))).clamp(-60000, 60000)      # (one head: no part past 6e4)
+    bounds = torch.stack([a.normal(a.N, 1, D) - 1, a.normal(a.N, 1, D) + 1], 2)
+    assert query.float().abs().sum((1, 2)).amin() > 6e4 and query.float().abs().sum(1).amax() < 6e4
+    lib = _cabi.load()
+    for overflow in (False, True):
+        if overflow:
+            query[:, :, 0] = 60000.0 / min(group, 2) + 3000.0
+        want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, k, 1, 1)
+        q, b, table, lens, starts = on_gpu(query, bounds, a.table, a.lens, a.starts)
+        c = _cabi.PagedCache(page_table=table.data_ptr(), table_stride=table.stride(0), lens=lens.data_ptr(), starts=starts.data_ptr(),
+                             pages=a.N, kv_heads=1, page_size=16, dim=D, dtype=_cabi.FCS_DTYPE_FP16, sequences=1, table_width=pages, tokens=tokens)
+        room = torch.full((lib.fcs_select_pages_workspace_bytes(ctypes.byref(c)),), 0xab, dtype=torch.uint8, device="cuda")
+        out = torch.empty(tokens, 1, k, dtype=torch.int32, device="cuda")
+        stride = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
+        assert lib.fcs_select_pages(ctypes.byref(c), q.data_ptr(), stride, group, b.data_ptr(), k, 1, 1, out.data_ptr(), 1, room.data_ptr(),
+                                    room.numel(), ops._status_word(out.device).data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(out.cpu(), want)
+        sums = room[:8 * tokens * (pages + 4)].view(torch.int64)             # (a pitch of the next multiple of four)
+        written = (sums != int.from_bytes(b"\xab" * 8, "little", signed=True)).sum().item()
+        # (a token's competing pages: those it sees but the first and its own; 4 of 20 tokens lie in the last page but one)
+        assert written == (sum(pos // 16 - 1 for _, _, pos in places(a.lens, a.starts, tokens)) if overflow else 0)
     status_is(0)
