@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
     const long long s1 = c.starts[b + 1], t0 = s0 + (tile - (s0 / p.tile_tokens + b)) * p.tile_tokens;
     if (s0 < 0 || s1 > c.tokens || t0 < s0 || t0 >= s1) return;
     const int tokens = (int)min((long long)p.tile_tokens, s1 - t0);
-    const int pos0 = (int)min(position_of(c, b, (int)t0), 1ll << 30);          // of the first token (no table here is as long)
+    // of the first token (no table here is as long, and no block reaches back from there to a key)
+    const int pos0 = (int)max(min(position_of(c, b, (int)t0), 1ll << 30), -(1ll << 30));
     const int P = 1 << c.page_shift;
     const int pages = pos0 + tokens <= 0 ? 0 : (pos0 + tokens - 1 >> c.page_shift) + 1;      // that the last token sees
 

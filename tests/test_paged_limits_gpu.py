@@ -209,3 +209,24 @@ def test_large_queries_of_half_precision_need_no_more_sums_than_others(tokens, g
         # (a token's competing pages: those it sees but the first and its own; 4 of 20 tokens lie in the last page but one)
         assert written == (sum(pos // 16 - 1 for _, _, pos in places(a.lens, a.starts, tokens)) if overflow else 0)
     status_is(0)
+
+
+# --------------------------------------------------------------------------- lengths
+@pytest.mark.parametrize("tokens", [1, 20])           # a row at a time, and blocks of tokens
+@pytest.mark.parametrize("length", [-2 ** 31, -2 ** 31 + 4, -2 ** 31 + 19, -1, 0])
+def test_tokens_in_front_of_a_sequence_see_nothing(tokens, length):
+    """Lengths that count fewer tokens than there are rows, down to the lowest: no key is seen, no page chosen, nothing is written."""
+    import flash_colsum_b200 as fc
+    a = Batch(39, [tokens], [16 * 8], 16, 1, 1, 64, BF16)
+    q, k, kp, vp, table, starts = on_gpu(a.rows(1), a.rows(1), a.pool(), a.pool(), a.table, a.starts)
+    lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+    pages = torch.arange(8, dtype=torch.int32, device="cuda").expand(tokens, 1, 8)
+    out, lse = fc.attend_pages(q, kp, vp, table, lens, pages, starts=starts, return_lse=True)
+    assert (out == 0).all() and (lse == -torch.inf).all()
+    bounds = torch.stack([kp.amin(2), kp.amax(2)], 2)
+    assert (fc.select_pages(q, bounds, table, lens, 3, page_size=16, starts=starts) == -1).all()
+    status_is(0)
+    before = [t.clone() for t in (kp, vp, bounds)]
+    fc.append_paged(k, k, kp, vp, table, lens, starts=starts, bounds=bounds)
+    assert all(torch.equal(x, y) for x, y in zip(before, (kp, vp, bounds)))
+    status_is(5)
