@@ -24,9 +24,10 @@ EXPORTED_SYMBOLS = (
     "fcs_selftest_wait_expiry_cluster",
     "fcs_peer_post", "fcs_peer_wait", "fcs_colsum_causal_accumulate_signalled",
     "fcs_append_paged", "fcs_select_pages", "fcs_select_pages_workspace_bytes", "fcs_attend_pages",
+    "fcs_selftest_wait_expiry_select", "fcs_selftest_wait_expiry_attend",
 )
 
-ABI_VERSION = 203   # fcs_version() of the library these argument lists were written for
+ABI_VERSION = 204   # fcs_version() of the library these argument lists were written for
 FCS_OK = 0
 FCS_ERR_UNSUPPORTED = -2
 FCS_DTYPE_FP16 = 0
@@ -154,6 +155,11 @@ def load() -> ctypes.CDLL:
     lib.fcs_select_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _i, _i, _p, _i, _p, _sz, _p, _p]
     lib.fcs_attend_pages.restype = _i
     lib.fcs_attend_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _f, _p, ctypes.POINTER(_i64), _p, _i, _p, _p]
+    lib.fcs_selftest_wait_expiry_select.restype = _i
+    lib.fcs_selftest_wait_expiry_select.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _i, _i, _p, _p, _sz, _p, ctypes.c_double, _p]
+    lib.fcs_selftest_wait_expiry_attend.restype = _i
+    lib.fcs_selftest_wait_expiry_attend.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _f, _p, ctypes.POINTER(_i64), _p, _p,
+                                                    ctypes.c_double, _p]
     lib.fcs_set_profiling.restype = _i
     lib.fcs_set_profiling.argtypes = [_i]
     lib.fcs_set_single_pass.restype = _i

@@ -2181,7 +2181,7 @@ static int static_scratch_address(void** out_ptr) {
 // ---------------------------------------------------------------------------
 extern "C" {
 
-int fcs_version(void) { return 203; }
+int fcs_version(void) { return 204; }
 
 const char* fcs_last_error(void) { return fcs::g_err; }
 

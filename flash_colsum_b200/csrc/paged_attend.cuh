@@ -45,6 +45,7 @@ struct AttendParams {
     int tile_tokens;               // (attend_shared_kernel) tokens of a CTA
     float c_log2;                  // scale * log2(e)
     int fill_tail;                 // rows behind the last sequence: 1 zeros the output's, 2 sets the sums' to -inf
+    int withhold;                  // (self-test) the producer issues nothing
 };
 
 template <int DP, int STAGES>
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
         const int e1 = min(p.k, (int)((long long)units * (rank + 1) / CL) * per_tile);
         const int* list = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
         int stage = 0, phase = 1, place = 0;
-        bool fine = true;
+        bool fine = !p.withhold;
         const uint32_t piece = (uint32_t)place_keys * 128u;
         for (int base = e0; base < e1 && fine; base += 32) {
             const int e = base + lane;
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
 
     // The ring goes on from pass to pass: one over the sets, and if need be one over each token's own list.
     int stage = 0, phase = warp == SHARED_WARPS ? 1 : 0;
-    bool fine = true;
+    bool fine = warp < SHARED_WARPS || !p.withhold;
     int pass = twice ? 0 : -1;
     while (true) {
         Columns<KS, NT, BF16> have;

@@ -45,6 +45,7 @@ struct SelectParams {
     int pitch, splits;
     int t0, t1;                     // tokens of this launch
     int fill_tail;
+    int withhold;                   // (self-test) no bounds are asked for
 };
 
 template <bool BF16>
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     // This warp's next 16 pages; whether each is one of the pools'.  (For one that is not, page 0 stands in.)
     auto ask = [&](int first, int entry) {
         const int n = min(16, end - first);
-        if (n <= 0) return;
+        if (n <= 0 || p.withhold) return;
         if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * 4 * D));
         __syncwarp();
         if (lane < n) {

@@ -304,7 +304,7 @@ static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t
 
 static int select(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const void* bounds,
                   int k, int first, int last, int* chosen, int fill_tail, void* workspace, size_t workspace_bytes, int* status,
-                  cudaStream_t stream) {
+                  cudaStream_t stream, bool withhold = false) {
     SelectParams p;
     memset(&p, 0, sizeof(p));
     int rc = check_cache(cache, p.c, status);
@@ -317,6 +317,7 @@ static int select(const FcsPagedCache* cache, const void* query, const int64_t* 
     if (k < 1 || first < 0 || last < 1 || (long long)first + last > k)
         return fail(FCS_ERR_INVALID_ARGUMENT, "k must hold the first and the last pages (k=%d first=%d last=%d)", k, first, last);
     const SelectPlan plan = select_plan(cache);
+    if (withhold && plan.tiles) return fail(FCS_ERR_UNSUPPORTED, "this call has no waits");
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < plan.bytes)
         return fail(FCS_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes, got %zu", plan.bytes, workspace_bytes);
     p.query = static_cast<const uint16_t*>(query);
@@ -334,6 +335,7 @@ static int select(const FcsPagedCache* cache, const void* query, const int64_t* 
     p.pitch = (int)plan.pitch;
     p.splits = plan.splits;
     p.fill_tail = fill_tail;
+    p.withhold = withhold;
     for (long long t0 = 0; t0 < cache->tokens; t0 += plan.at_once) {
         p.t0 = (int)t0;
         p.t1 = (int)(cache->tokens - t0 < plan.at_once ? cache->tokens : t0 + plan.at_once);
@@ -419,7 +421,8 @@ static int cluster_for(long long rows, int per_sm, int most) {
 }
 
 static int attend(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const int* chosen, int k,
-                  float scale, void* out, const int64_t* out_stride, float* lse, int fill_tail, int* status, cudaStream_t stream) {
+                  float scale, void* out, const int64_t* out_stride, float* lse, int fill_tail, int* status, cudaStream_t stream,
+                  bool withhold = false) {
     AttendParams p;
     memset(&p, 0, sizeof(p));
     int rc = check_cache(cache, p.c, status);
@@ -449,6 +452,7 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     p.q_heads = q_heads;
     p.c_log2 = scale * 1.4426950408889634f;
     p.fill_tail = fill_tail;
+    p.withhold = withhold;
     const bool wide = cache->dim > 64, bf16 = cache->dtype == FCS_DTYPE_BF16;
     CUtensorMap km, vm;
     if ((rc = pool_map(&km, cache, cache->key_pages, cache->key_stride)) != FCS_OK) return rc;
@@ -487,6 +491,22 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     return FCS_OK;
 }
 
+// ------------------------------------------------------------------ waits that run out
+// `call` under a lower limit of the waits, for the self-tests.
+template <typename F>
+static int under_limit(double seconds, const int* status, cudaStream_t stream, F call) {
+    if (!status) return fail(FCS_ERR_INVALID_ARGUMENT, "status must not be NULL");
+    if (!(seconds > 0.0) || seconds > 2.0) return fail(FCS_ERR_INVALID_ARGUMENT, "limit_seconds must be in (0, 2]");
+    static long long short_limit, full_limit = kWaitLimitCycles;
+    short_limit = (long long)(seconds * 1.9e9);
+    cudaError_t e = cudaMemcpyToSymbolAsync(g_wait_limit_cycles, &short_limit, sizeof(long long), 0, cudaMemcpyHostToDevice, stream);
+    if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "the limit of the waits could not be set: %s", cudaGetErrorString(e));
+    const int rc = call();
+    e = cudaMemcpyToSymbolAsync(g_wait_limit_cycles, &full_limit, sizeof(long long), 0, cudaMemcpyHostToDevice, stream);
+    if (rc == FCS_OK && e != cudaSuccess) return fail(FCS_ERR_CUDA, "the limit of the waits could not be set back: %s", cudaGetErrorString(e));
+    return rc;
+}
+
 }  // namespace paged
 }  // namespace fcs
 
@@ -515,6 +535,27 @@ int fcs_attend_pages(const FcsPagedCache* cache, const void* query, const int64_
     fcs::g_err[0] = 0;
     return fcs::paged::attend(cache, query, query_stride, q_heads, chosen, k, scale, out, out_stride, lse, fill_tail, status,
                               reinterpret_cast<cudaStream_t>(stream));
+}
+
+int fcs_selftest_wait_expiry_select(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads,
+                                    const void* bounds, int k, int first, int last, int* chosen, void* workspace,
+                                    size_t workspace_bytes, int* status, double limit_seconds, void* stream_v) {
+    fcs::g_err[0] = 0;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+    return fcs::paged::under_limit(limit_seconds, status, stream, [&] {
+        return fcs::paged::select(cache, query, query_stride, q_heads, bounds, k, first, last, chosen, 0, workspace, workspace_bytes,
+                                  status, stream, true);
+    });
+}
+
+int fcs_selftest_wait_expiry_attend(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads,
+                                    const int* chosen, int k, float scale, void* out, const int64_t* out_stride, float* lse,
+                                    int* status, double limit_seconds, void* stream_v) {
+    fcs::g_err[0] = 0;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+    return fcs::paged::under_limit(limit_seconds, status, stream, [&] {
+        return fcs::paged::attend(cache, query, query_stride, q_heads, chosen, k, scale, out, out_stride, lse, 0, status, stream, true);
+    });
 }
 
 }  // extern "C"

@@ -52,7 +52,8 @@ def _load_native(device: torch.device):
 
 
 def device_status(device=None) -> int:
-    """Synchronise and return the device status word (0 = no kernel gave up a wait)."""
+    """Synchronise and return the device status word, which keeps the first code of: 1 to 4, a kernel gave up a wait; 5, a call over a
+    paged cache needed a page that the table does not have; 6, a position that the rotation's tables do not have.  0: none did."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     return int(_status_word(dev).item())
 

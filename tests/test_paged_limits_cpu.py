@@ -1,9 +1,11 @@
 """What the entry points over a paged cache refuse at their limits, before anything is launched.  No GPU needed."""
 
+import ctypes
+
 import pytest
 
 from flash_colsum_b200 import _cabi
-from test_paged_cpu import append, attend, cache, rows
+from test_paged_cpu import ADDRESS, append, attend, cache, rows, strides
 
 
 @pytest.mark.parametrize("k", [2 ** 26 + 1, 2 ** 27, 2 ** 31 - 1])
@@ -27,3 +29,14 @@ def test_results_whose_rows_do_not_are_checked_further(tokens, heads, stride):
     c = cache(tokens=tokens, kv_heads=1)
     assert attend(c, heads=heads, out_st=stride, k=0) < 0
     assert "chosen" in _cabi.last_error()
+
+
+@pytest.mark.parametrize("changes,word", [(dict(status=None), "status"), (dict(limit=0.0), "limit_seconds"), (dict(limit=2.5), "limit_seconds")])
+def test_the_selftests_of_the_waits_check_their_arguments(changes, word):
+    limit, status = changes.get("limit", 0.05), changes.get("status", ADDRESS)
+    lib, c = _cabi.load(), ctypes.byref(cache())
+    assert lib.fcs_selftest_wait_expiry_select(c, ADDRESS, strides(1024, 128), 8, ADDRESS, 4, 1, 1, ADDRESS, ADDRESS, 1 << 40, status, limit, None) < 0
+    assert word in _cabi.last_error()
+    assert lib.fcs_selftest_wait_expiry_attend(c, ADDRESS, strides(1024, 128), 8, ADDRESS, 4, 0.1, ADDRESS, strides(1024, 128), None, status, limit,
+                                               None) < 0
+    assert word in _cabi.last_error()

@@ -1,5 +1,7 @@
 """What the entry points over a paged cache do at their limits: pages that the table lacks, the largest lists, results in odd memory."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -176,6 +178,18 @@ def test_autograd_sees_what_the_calls_write():
     status_is(0)
 
 
+def c_cache(a, table, lens, starts, pools=()):
+    """The batch (and contiguous pools) as the C entries take it; the tensors have to outlive it."""
+    from flash_colsum_b200 import _cabi
+    c = _cabi.PagedCache(page_table=table.data_ptr(), table_stride=table.stride(0), lens=lens.data_ptr(), starts=starts.data_ptr(),
+                         pages=a.N, kv_heads=a.H, page_size=a.P, dim=a.dim, dtype=0 if a.dtype == FP16 else 1, sequences=lens.numel(),
+                         table_width=table.shape[1], tokens=a.T)
+    if pools:
+        c.key_pages, c.value_pages = (p.data_ptr() for p in pools)
+        c.key_stride = c.value_stride = pools[0].stride()[:3]
+    return c
+
+
 # --------------------------------------------------------------------------- sums in 64 bits
 @pytest.mark.parametrize("tokens", [2, 20])           # a cluster a row, and tiles
 @pytest.mark.parametrize("group,D,size", [(32, 128, 20.0), (8, 128, 80.0), (4, 64, 1500.0), (1, 64, 2.0 ** 15)])
@@ -183,7 +197,6 @@ def test_large_queries_of_half_precision_need_no_more_sums_than_others(tokens, g
     """Parts whose magnitudes sum up to more than fp16 holds, each of them within its range: the 64-bit sums that the workspace has
     room for stay unwritten but for rows with many pages next to the border.  Parts past it: all are."""
     from flash_colsum_b200 import _cabi, ops
-    import ctypes
     pages, k = 500, 24
     a = Batch(38, [tokens], [16 * pages], 16, 1, group, D, FP16)
     query = a.rows(group)
@@ -196,8 +209,7 @@ def test_large_queries_of_half_precision_need_no_more_sums_than_others(tokens, g
             query[:, :, 0] = 60000.0 / min(group, 2) + 3000.0
         want = chosen_pages(query, bounds, 16, a.table, a.lens, a.starts, k, 1, 1)
         q, b, table, lens, starts = on_gpu(query, bounds, a.table, a.lens, a.starts)
-        c = _cabi.PagedCache(page_table=table.data_ptr(), table_stride=table.stride(0), lens=lens.data_ptr(), starts=starts.data_ptr(),
-                             pages=a.N, kv_heads=1, page_size=16, dim=D, dtype=_cabi.FCS_DTYPE_FP16, sequences=1, table_width=pages, tokens=tokens)
+        c = c_cache(a, table, lens, starts)
         room = torch.full((lib.fcs_select_pages_workspace_bytes(ctypes.byref(c)),), 0xab, dtype=torch.uint8, device="cuda")
         out = torch.empty(tokens, 1, k, dtype=torch.int32, device="cuda")
         stride = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
@@ -230,3 +242,61 @@ def test_tokens_in_front_of_a_sequence_see_nothing(tokens, length):
     fc.append_paged(k, k, kp, vp, table, lens, starts=starts, bounds=bounds)
     assert all(torch.equal(x, y) for x, y in zip(before, (kp, vp, bounds)))
     status_is(5)
+
+
+# --------------------------------------------------------------------------- waits that run out
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,pages,H", [(1, 40, 2), (2, 1100, 1), (150, 70, 8)])     # one CTA a row, sixteen, and one with others beside it
+def test_a_selection_whose_bounds_never_come_returns(rows, pages, H, D):
+    """No copy is issued and the limit is 50 ms: the waits run out, every CTA returns, the status word says so, what is written are
+    pages of the sequences; and the same call chooses as before."""
+    from flash_colsum_b200 import _cabi
+    lib, k = _cabi.load(), 9
+    a = Batch(40, [1] * rows, [16 * pages - i % 7 for i in range(rows)], 16, H, H, D, BF16)
+    query = a.rows(H)
+    bounds = torch.stack([a.normal(a.N, H, D) - 1, a.normal(a.N, H, D) + 1], 2)
+    first = select(a, query, bounds, k, 1, 1)
+    q, b, table, lens, starts = on_gpu(query, bounds, a.table, a.lens, a.starts)
+    c = c_cache(a, table, lens, starts)
+    room = torch.empty(lib.fcs_select_pages_workspace_bytes(ctypes.byref(c)), dtype=torch.uint8, device="cuda")
+    around = torch.full((rows * H * k + 512,), 7, dtype=torch.int32, device="cuda")
+    out, word = around[256:-256], torch.zeros(1, dtype=torch.int32, device="cuda")
+    stride = (ctypes.c_int64 * 2)(q.stride(0), q.stride(1))
+    assert lib.fcs_selftest_wait_expiry_select(ctypes.byref(c), q.data_ptr(), stride, H, b.data_ptr(), k, 1, 1, out.data_ptr(), room.data_ptr(),
+                                               room.numel(), word.data_ptr(), 0.05, torch.cuda.current_stream().cuda_stream) == 0, _cabi.last_error()
+    torch.cuda.synchronize()
+    assert int(word) == 3                        # FCS_STATUS_WAIT_CONSUMER
+    assert int(out.amin()) >= -1 and int(out.amax()) < pages
+    assert (around[:256] == 7).all() and (around[-256:] == 7).all()
+    assert torch.equal(select(a, query, bounds, k, 1, 1), first)
+    status_is(0)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("tokens,H,k,twice", [(1, 1, 2, False), (1, 1, 300, False), (300, 1, 3, False), (40, 1, 7, False), (40, 1, 7, True),
+                                              (40, 100, 7, True)])
+def test_an_attention_whose_pages_never_come_returns(tokens, H, k, twice, D):
+    """A row at a time over one CTA and sixteen, blocks of tokens over eight and two, also where a list names a page twice and every
+    token has a pass of its own: zeros and -inf, and a status; and the same call attends as before."""
+    import flash_colsum_b200 as fc
+    from flash_colsum_b200 import _cabi
+    lib = _cabi.load()
+    many = tokens == 300                          # sequences of one token
+    a = Batch(41, [1] * tokens if many else [tokens], [16 * 20 + tokens] * (tokens if many else 1), 16, H, H, D, BF16, width=400)
+    query, kp, vp, table, lens, starts = on_gpu(a.rows(H), a.pool(), a.pool(), a.table, a.lens, a.starts)
+    pages = torch.randperm(20, generator=a.g).int()[torch.arange(k) % 20].expand(a.T, H, k).contiguous().cuda()
+    if twice:
+        pages[:, :, 0] = pages[:, :, 1]
+    first = fc.attend_pages(query, kp, vp, table, lens, pages, starts=starts, return_lse=True)
+    c = c_cache(a, table, lens, starts, (kp, vp))
+    out, lse = torch.full_like(query, 7.0), torch.full((a.T, H), 7.0, device="cuda")
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    stride = (ctypes.c_int64 * 2)(query.stride(0), query.stride(1))
+    assert lib.fcs_selftest_wait_expiry_attend(ctypes.byref(c), query.data_ptr(), stride, H, pages.data_ptr(), k, 0.1, out.data_ptr(), stride,
+                                               lse.data_ptr(), word.data_ptr(), 0.05, torch.cuda.current_stream().cuda_stream) == 0, _cabi.last_error()
+    torch.cuda.synchronize()
+    assert int(word) == 3
+    assert (out == 0).all() and (lse == -torch.inf).all()
+    again = fc.attend_pages(query, kp, vp, table, lens, pages, starts=starts, return_lse=True)
+    assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    status_is(0)
