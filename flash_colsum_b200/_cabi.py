@@ -24,7 +24,7 @@ EXPORTED_SYMBOLS = (
     "fcs_selftest_wait_expiry_cluster",
     "fcs_peer_post", "fcs_peer_wait", "fcs_colsum_causal_accumulate_signalled",
     "fcs_append_paged", "fcs_select_pages", "fcs_select_pages_workspace_bytes", "fcs_attend_pages",
-    "fcs_selftest_wait_expiry_select", "fcs_selftest_wait_expiry_attend",
+    "fcs_selftest_wait_expiry_select", "fcs_selftest_wait_expiry_attend", "fcs_paged_plan",
 )
 
 ABI_VERSION = 204   # fcs_version() of the library these argument lists were written for
@@ -60,6 +60,12 @@ class PagedRows(ctypes.Structure):
                 ("query_out_stride", _i64 * 2), ("q_heads", _i), ("cos", _p), ("sin", _p),
                 ("table_rows", _i), ("rotary", _i), ("interleaved", _i), ("positions", _p), ("bounds", _p),
                 ("fill_tail", _i)]
+
+
+class PagedPlan(ctypes.Structure):
+    """`FcsPagedPlan` of the header."""
+    _fields_ = [(name, _i) for name in ("append_heads", "append_steps", "select_tiles", "select_ctas", "select_launches",
+                                        "attend_tokens", "attend_queries", "attend_ctas")]
 
 
 class LibraryMissing(RuntimeError):
@@ -155,6 +161,8 @@ def load() -> ctypes.CDLL:
     lib.fcs_select_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _i, _i, _p, _i, _p, _sz, _p, _p]
     lib.fcs_attend_pages.restype = _i
     lib.fcs_attend_pages.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _f, _p, ctypes.POINTER(_i64), _p, _i, _p, _p]
+    lib.fcs_paged_plan.restype = _i
+    lib.fcs_paged_plan.argtypes = [cache, _i, _i, ctypes.POINTER(PagedPlan)]
     lib.fcs_selftest_wait_expiry_select.restype = _i
     lib.fcs_selftest_wait_expiry_select.argtypes = [cache, _p, ctypes.POINTER(_i64), _i, _p, _i, _i, _i, _p, _p, _sz, _p, ctypes.c_double, _p]
     lib.fcs_selftest_wait_expiry_attend.restype = _i
@@ -286,3 +294,11 @@ def plan_info(B: int, H: int, sq_rows: int, Sk: int, is_causal: bool) -> dict:
         raise RuntimeError("fcs_plan_info rejected the sizes")
     return {"nsplit": nsplit.value, "stats_items": items.value, "colsum_steps": steps.value,
             "sms": sms.value}
+
+
+def paged_plan(cache: PagedCache, q_heads: int, k: int) -> dict:
+    """What calls over a paged cache launch for a batch of these sizes."""
+    plan = PagedPlan()
+    if load().fcs_paged_plan(ctypes.byref(cache), q_heads, k, ctypes.byref(plan)) != FCS_OK:
+        raise RuntimeError(f"fcs_paged_plan rejected the sizes: {last_error()}")
+    return {name: getattr(plan, name) for name, _ in PagedPlan._fields_}

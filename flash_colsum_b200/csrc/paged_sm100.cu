@@ -146,6 +146,23 @@ static cudaError_t launch_append(int rot, dim3 grid, cudaStream_t stream, const 
                       : launch(append_kernel<Ops, 2>, grid, APPEND_THREADS, 0, 1, stream, p);
 }
 
+struct AppendPlan {
+    int heads_shift, steps;
+};
+
+// A CTA has about 32 rows at a time, the heads of a group times the tokens of a page.  Of long calls it has more of the values
+// and queries, whose heads share a token's rotation: 16384 tokens, 32 and 8 heads 121 us with one step, 78 with two, 76 with
+// four; 1861 tokens of 7 sequences, 16 and 16 heads, pages of 16 13.2 us with one, 11.2 with two, 12.0 with four.
+static AppendPlan append_plan(const FcsPagedCache* cache, int q_heads) {
+    AppendPlan a = {0, 1};
+    const long long B = cache->sequences, T = cache->tokens, P = cache->page_size;
+    const long long each = cache->starts ? (T / B < P ? (T + B - 1) / B : P) : 1;
+    while (a.heads_shift < 3 && (each << a.heads_shift) < 32) ++a.heads_shift;
+    const long long ctas = T / each * (q_heads + cache->kv_heads) / (1 << a.heads_shift);
+    a.steps = ctas >= 32ll * num_sms() ? 4 : ctas >= 8ll * num_sms() ? 2 : 1;
+    return a;
+}
+
 static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status, cudaStream_t stream) {
     AppendParams p;
     memset(&p, 0, sizeof(p));
@@ -197,15 +214,11 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
     }
     p.q_heads = with_query ? r->q_heads : 0;
     p.fill_tail = r->fill_tail != 0;
-    // A CTA has about 32 rows at a time, the heads of a group times the tokens of a page.  Of long calls it has more of the values
-    // and queries, whose heads share a token's rotation: 16384 tokens, 32 and 8 heads 121 us with one step, 78 with two, 76 with
-    // four; 1861 tokens of 7 sequences, 16 and 16 heads, pages of 16 13.2 us with one, 11.2 with two, 12.0 with four.
-    const long long B = cache->sequences, T = cache->tokens, P = cache->page_size;
-    const long long each = cache->starts ? (T / B < P ? (T + B - 1) / B : P) : 1;
-    while (p.heads_shift < 3 && (each << p.heads_shift) < 32) ++p.heads_shift;
+    const AppendPlan plan = append_plan(cache, p.q_heads);
+    p.heads_shift = plan.heads_shift;
+    p.steps = plan.steps;
     const int heads = 1 << p.heads_shift;
-    const long long ctas = T / each * (p.q_heads + cache->kv_heads) / heads;
-    p.steps = ctas >= 32ll * num_sms() ? 4 : ctas >= 8ll * num_sms() ? 2 : 1;
+    const long long B = cache->sequences, T = cache->tokens, P = cache->page_size;
     p.key_groups = (cache->kv_heads + heads - 1) / heads;
     p.value_groups = (cache->kv_heads + heads * p.steps - 1) / (heads * p.steps);
     const long long segments = cache->starts ? T / P + 2 * B + 1 : B;
@@ -259,6 +272,19 @@ static SelectPlan select_plan(const FcsPagedCache* c) {
     return s;
 }
 
+template <bool BF16>
+static int widest_row_cluster() {
+    static int known[64] = {0};
+    return sixteen_fit(known, select_row_kernel<BF16, 128, 16>, ROW_THREADS, row_smem(128, ROW_PAGES)) ? 16 : 8;
+}
+
+// CTAs of a row (select_row_kernel): as many as the device runs at once, 64 pages for each at least.
+static int row_ctas(long long rows, int width, int widest) {
+    int cl = 1;
+    while (cl < widest && rows * cl * 2 <= (long long)ROW_CTAS * num_sms() && width >= 128 * cl) cl *= 2;
+    return cl;
+}
+
 template <bool BF16, int DP, int CL>
 static cudaError_t launch_select_row(const SelectParams& p, unsigned tokens, cudaStream_t stream) {
     static bool done[64] = {false};
@@ -280,12 +306,7 @@ template <bool BF16>
 static cudaError_t launch_select(const SelectParams& p, bool tiles, cudaStream_t stream) {
     const unsigned tokens = (unsigned)(p.t1 - p.t0);
     if (!tiles) {
-        // CTAs of a row: as many as the device runs at once, 64 pages for each at least
-        const long long rows = (long long)tokens * p.c.kv_heads;
-        int cl = 1;
-        static int known[64] = {0};
-        const int widest = sixteen_fit(known, select_row_kernel<BF16, 128, 16>, ROW_THREADS, row_smem(128, ROW_PAGES)) ? 16 : 8;
-        while (cl < widest && rows * cl * 2 <= (long long)ROW_CTAS * num_sms() && p.c.width >= 128 * cl) cl *= 2;
+        const int cl = row_ctas((long long)tokens * p.c.kv_heads, p.c.width, widest_row_cluster<BF16>());
         return p.c.dim > 64 ? launch_select_cl<BF16, 128>(cl, p, tokens, stream) : launch_select_cl<BF16, 64>(cl, p, tokens, stream);
     }
     static bool done[64] = {false};
@@ -420,6 +441,34 @@ static int cluster_for(long long rows, int per_sm, int most) {
     return best;
 }
 
+struct AttendPlan {
+    bool shared;             // tokens share their pages (attend_shared_kernel)
+    int tile_tokens;         // tokens of a block, then
+    int nt, query_tiles;     // a row at a time: sets of eight queries in a CTA, and CTAs over a row's queries
+    int cl;                  // CTAs of a block or row
+};
+
+// Tokens of a sequence share what they chose in common, where there are enough of them: more than two a sequence, and blocks
+// for all SMs or of eight tokens.  Measured, blocks against a token at a time, 32 pages of 64 for groups of four heads: 512
+// blocks of two tokens 127 and 121 us; 256 of four 96 and 105, 192 of four 50 and 62; 128 of four 48 and 42 (58 and 52), 64
+// of four 34 and 22; heads of their own, 64 of sixteen 53 and 60, 32 of sixteen 29 and 39.
+static AttendPlan attend_plan(const FcsPagedCache* cache, int group, int k) {
+    AttendPlan a;
+    const long long T = cache->tokens, B = cache->sequences;
+    a.tile_tokens = SHARED_COLS / group < 31 ? SHARED_COLS / group : 31;
+    const long long blocks = (a.tile_tokens > 0 && T / a.tile_tokens > B ? T / a.tile_tokens : B) * cache->kv_heads;
+    const long long together = T / B < a.tile_tokens ? T / B : a.tile_tokens;
+    a.shared = cache->starts && T > 2 * B && a.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES &&
+               (blocks >= num_sms() || together >= 8);
+    a.nt = group > 8 ? 2 : 1;
+    a.query_tiles = (group + 8 * a.nt - 1) / (8 * a.nt);
+    const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
+    a.cl = a.shared ? cluster_for(blocks, cache->dim > 64 ? SHARED_CTAS<128> : SHARED_CTAS<64>, 8)
+                    : cluster_for(T * cache->kv_heads * a.query_tiles, 2,      // (two tiles of keys for each CTA at least)
+                                  tiles >= 32 ? 16 : tiles >= 16 ? 8 : tiles >= 8 ? 4 : tiles >= 4 ? 2 : 1);
+    return a;
+}
+
 static int attend(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads, const int* chosen, int k,
                   float scale, void* out, const int64_t* out_stride, float* lse, int fill_tail, int* status, cudaStream_t stream,
                   bool withhold = false) {
@@ -459,28 +508,19 @@ static int attend(const FcsPagedCache* cache, const void* query, const int64_t* 
     if ((rc = pool_map(&vm, cache, cache->value_pages, cache->value_stride)) != FCS_OK) return rc;
     cudaError_t e;
     const long long T = cache->tokens, B = cache->sequences;
-    p.tile_tokens = SHARED_COLS / p.group < 31 ? SHARED_COLS / p.group : 31;
-    // Tokens of a sequence share what they chose in common, where there are enough of them: more than two a sequence, and blocks
-    // for all SMs or of eight tokens.  Measured, blocks against a token at a time, 32 pages of 64 for groups of four heads: 512
-    // blocks of two tokens 127 and 121 us; 256 of four 96 and 105, 192 of four 50 and 62; 128 of four 48 and 42 (58 and 52), 64
-    // of four 34 and 22; heads of their own, 64 of sixteen 53 and 60, 32 of sixteen 29 and 39.
-    const long long blocks = (p.tile_tokens > 0 && T / p.tile_tokens > B ? T / p.tile_tokens : B) * cache->kv_heads;
-    const long long together = T / B < p.tile_tokens ? T / B : p.tile_tokens;
-    if (cache->starts && T > 2 * B && p.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES &&
-        (blocks >= num_sms() || together >= 8)) {
-        const int cl = cluster_for(blocks, wide ? SHARED_CTAS<128> : SHARED_CTAS<64>, 8);
+    const AttendPlan plan = attend_plan(cache, p.group, k);
+    const int cl = plan.cl;
+    if (plan.shared) {
+        p.tile_tokens = plan.tile_tokens;
         if (8 * (T / p.tile_tokens + B + 1) > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
         e = wide ? (bf16 ? launch_shared_cl<128, true>(cl, km, vm, p, stream) : launch_shared_cl<128, false>(cl, km, vm, p, stream))
                  : (bf16 ? launch_shared_cl<64, true>(cl, km, vm, p, stream) : launch_shared_cl<64, false>(cl, km, vm, p, stream));
         if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "attending failed to launch: %s", cudaGetErrorString(e));
         return FCS_OK;
     }
-    const int nt = p.group > 8 ? 2 : 1;
-    p.query_tiles = (p.group + 8 * nt - 1) / (8 * nt);
-    const long long rows = T * cache->kv_heads * p.query_tiles;
-    const long long tiles = ((long long)k * cache->page_size + TILE_KEYS - 1) / TILE_KEYS;
-    const int cl = cluster_for(rows, 2, tiles >= 32 ? 16 : tiles >= 16 ? 8 : tiles >= 8 ? 4 : tiles >= 4 ? 2 : 1);     // (two tiles of keys for each CTA at least)
-    if (rows / cache->kv_heads * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
+    const int nt = plan.nt;
+    p.query_tiles = plan.query_tiles;
+    if (T * p.query_tiles * cl > 0x7fffffffll) return fail(FCS_ERR_UNSUPPORTED, "too many tokens (%d) for one launch", cache->tokens);
     if (wide)
         e = nt == 1 ? (bf16 ? launch_attend_cl<128, 1, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 1, false>(cl, km, vm, p, stream))
                     : (bf16 ? launch_attend_cl<128, 2, true>(cl, km, vm, p, stream) : launch_attend_cl<128, 2, false>(cl, km, vm, p, stream));
@@ -535,6 +575,33 @@ int fcs_attend_pages(const FcsPagedCache* cache, const void* query, const int64_
     fcs::g_err[0] = 0;
     return fcs::paged::attend(cache, query, query_stride, q_heads, chosen, k, scale, out, out_stride, lse, fill_tail, status,
                               reinterpret_cast<cudaStream_t>(stream));
+}
+
+int fcs_paged_plan(const FcsPagedCache* cache, int q_heads, int k, FcsPagedPlan* plan) {
+    fcs::g_err[0] = 0;
+    using namespace fcs::paged;
+    Batch unused;
+    const int rc = check_cache(cache, unused, nullptr);
+    if (rc != FCS_OK) return rc;
+    if (!plan || q_heads < 0 || q_heads % cache->kv_heads || k < 1)
+        return fcs::fail(FCS_ERR_INVALID_ARGUMENT, "plan is NULL, or bad sizes (q_heads=%d k=%d)", q_heads, k);
+    memset(plan, 0, sizeof(*plan));
+    const AppendPlan a = append_plan(cache, q_heads);
+    plan->append_heads = 1 << a.heads_shift;
+    plan->append_steps = a.steps;
+    const SelectPlan s = select_plan(cache);
+    const long long at_once = s.at_once;
+    plan->select_tiles = s.tiles;
+    plan->select_launches = (int)((cache->tokens + at_once - 1) / at_once);
+    plan->select_ctas = s.tiles ? 1
+                                : row_ctas(at_once * cache->kv_heads, cache->table_width,
+                                           cache->dtype == FCS_DTYPE_BF16 ? widest_row_cluster<true>() : widest_row_cluster<false>());
+    if (q_heads == 0) return FCS_OK;
+    const AttendPlan t = attend_plan(cache, q_heads / cache->kv_heads, k);
+    plan->attend_tokens = t.shared ? t.tile_tokens : 1;
+    plan->attend_queries = t.shared ? SHARED_COLS : 8 * t.nt;
+    plan->attend_ctas = t.cl;
+    return FCS_OK;
 }
 
 int fcs_selftest_wait_expiry_select(const FcsPagedCache* cache, const void* query, const int64_t* query_stride, int q_heads,

@@ -526,6 +526,21 @@ int fcs_selftest_wait_expiry_attend(const FcsPagedCache *cache, const void *quer
 int fcs_plan_info(int B, int H, int sq_rows, int Sk, int is_causal, int *nsplit,
                   long long *stats_items, long long *colsum_steps, int *sms);
 
+/*
+ * The same for calls over a paged cache: what the three entries launch for a batch of these sizes on the current device (the
+ * pointers of `cache` are not followed, but must not be NULL where the entries want them; starts says whether there are any).
+ * q_heads 0: keys and values alone.
+ */
+typedef struct FcsPagedPlan {
+    int append_heads, append_steps;       /* heads that a CTA has at a time, and how often (values and queries) */
+    int select_tiles;                     /* 1: scores by tiles of 64 tokens; 0: a row at a time, over ... */
+    int select_ctas;                      /* ... a cluster of this many CTAs (of the first launch) */
+    int select_launches;                  /* (with tiles, pairs of them) */
+    int attend_tokens, attend_queries;    /* tokens that share their pages in a CTA, its columns */
+    int attend_ctas;                      /* CTAs of a cluster (16: or 8, where the device cannot hold sixteen) */
+} FcsPagedPlan;
+int fcs_paged_plan(const FcsPagedCache *cache, int q_heads, int k, FcsPagedPlan *plan);
+
 #ifdef __cplusplus
 }
 #endif

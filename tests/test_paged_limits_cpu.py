@@ -40,3 +40,23 @@ def test_the_selftests_of_the_waits_check_their_arguments(changes, word):
     assert lib.fcs_selftest_wait_expiry_attend(c, ADDRESS, strides(1024, 128), 8, ADDRESS, 4, 0.1, ADDRESS, strides(1024, 128), None, status, limit,
                                                None) < 0
     assert word in _cabi.last_error()
+
+
+def test_plans_of_calls_over_a_paged_cache():
+    """Host arithmetic, of 148 SMs where there is no device."""
+    c = cache(sequences=32, tokens=32, starts=None, kv_heads=8, table_width=512, table_stride=512)
+    p = _cabi.paged_plan(c, 32, 32)
+    assert (p["append_heads"], p["append_steps"]) == (8, 1)
+    assert (p["select_tiles"], p["select_ctas"], p["select_launches"]) == (0, 2, 1)
+    assert (p["attend_tokens"], p["attend_queries"], p["attend_ctas"]) == (1, 8, 1)
+    c = cache(sequences=1, tokens=512, kv_heads=8, table_width=512, table_stride=512)
+    p = _cabi.paged_plan(c, 32, 32)
+    assert p["select_tiles"] == 1 and (p["attend_tokens"], p["attend_ctas"]) == (4, 1)
+    assert _cabi.paged_plan(cache(sequences=1, tokens=16384, kv_heads=8), 32, 1)["append_steps"] == 4
+    assert _cabi.paged_plan(cache(sequences=1, tokens=1000, kv_heads=8, table_width=8192, table_stride=8192), 32, 48)["select_launches"] == 3
+    assert _cabi.paged_plan(c, 0, 1)["attend_ctas"] == 0
+    for heads, k in ((7, 1), (-8, 1), (8, 0)):
+        with pytest.raises(RuntimeError, match="rejected"):
+            _cabi.paged_plan(c, heads, k)
+    with pytest.raises(RuntimeError, match="page size"):
+        _cabi.paged_plan(cache(page_size=8), 8, 1)
