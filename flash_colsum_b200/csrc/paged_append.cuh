@@ -34,7 +34,7 @@ struct AppendParams {
     long long key_page_st[3], value_page_st[3];                       // page, head, slot
     const float *cos, *sin;        // (table_rows, rotary / 2)
     const int* positions;          // or nullptr: where the token lies in its sequence
-    int q_heads, rotary, interleaved, table_rows;
+    int q_heads, rotary, table_rows;
     int heads_shift;               // heads that a CTA has at a time, as a power of two (at most 16)
     int steps;                     // and how often, of values and queries
     int key_groups, value_groups;  // CTAs over the key heads, over the value heads

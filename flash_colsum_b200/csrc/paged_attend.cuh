@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
 
 // ------------------------------------------------------------------ many tokens a sequence
 // Neighbouring tokens choose many pages in common, and what bounds them is the fetching.  So a CTA has several of them, as many as
-// fit its columns (31 at most): the pages that any of them chose, in a table of token sets, are fetched once, and eight columns
+// fit its sixteen columns: the pages that any of them chose, in a table of token sets, are fetched once, and eight columns
 // whose tokens did not choose a page pass over it.  What a token did not choose is masked from its columns -- but 0 times a
 // value that is not finite is not 0, so a result that is not finite is formed again from the token's own pages alone, as are
 // those of a list that names a page twice.
@@ -457,9 +457,9 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
 // at a time 284 us and 4.3 GB through L2; 16 columns, four tokens, 2.2 GB and 190 us with three CTAs per SM (two stages of tiles),
 // 210 us with two (three stages); 32 columns 240 us and 48 or 64 columns 230 and 236 us, one CTA per SM.  57 tokens in threes, 64
 // pages of 16 keys, heads of 64: 74 us, with four CTAs per SM 55.
-constexpr int SHARED_GROUPS = 1, SHARED_NT = 2;
-constexpr int SHARED_COLS = SHARED_GROUPS * SHARED_NT * 8;
-constexpr int SHARED_WARPS = 4 * SHARED_GROUPS;        // consumers
+constexpr int SHARED_NT = 2;
+constexpr int SHARED_COLS = SHARED_NT * 8;
+constexpr int SHARED_WARPS = 4;                        // consumers
 constexpr int SHARED_THREADS = (SHARED_WARPS + 1) * 32;
 constexpr int SHARED_PAGES = 8192;                     // of the table of token sets
 template <int DP> constexpr int SHARED_CTAS = DP == 128 ? 3 : 4;      // per SM
@@ -629,24 +629,23 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
             }
         } else {
             // ---- consumers
-            const int group = warp >> 2, quarter = warp & 3;
             int tok[NT][2];            // of this thread's columns; 31: of nobody
             uint32_t mine[NT];         // the tokens of eight columns
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int k = ((group * NT + n) * 8 + 2 * (lane & 3) + j) / G;
+                    const int k = (n * 8 + 2 * (lane & 3) + j) / G;
                     tok[n][j] = k < tokens ? k : 31;
                 }
                 mine[n] = __reduce_or_sync(0xffffffffu, 1u << tok[n][0] | 1u << tok[n][1]) & 0x7fffffffu;
             }
             const int place_keys = P < TILE_KEYS ? P : TILE_KEYS;
-            const int my_place = quarter * 16 / place_keys, my_off = quarter * 16 % place_keys;
-            const int key_row = quarter * 16 + (lane & 15), val_row = quarter * 16 + (lane >> 4) * 8 + (lane & 7);
+            const int my_place = warp * 16 / place_keys, my_off = warp * 16 % place_keys;
+            const int key_row = warp * 16 + (lane & 15), val_row = warp * 16 + (lane >> 4) * 8 + (lane & 7);
             const uint32_t key_at = tiles + key_row * 128 + (((lane >> 4) ^ (key_row & 7)) << 4);
             const uint32_t val_at = tiles + L::SLABS * SLAB_BYTES + val_row * 128 + ((((lane >> 3) & 1) ^ (val_row & 7)) << 4);
-            const uint32_t q_at = tiles + L::OFF_Q + (group * NT * 8 + (lane & 7) + (lane >> 4) * 8) * L::Q_PITCH + ((lane >> 3) & 1) * 16;
+            const uint32_t q_at = tiles + L::OFF_Q + ((lane & 7) + (lane >> 4) * 8) * L::Q_PITCH + ((lane >> 3) & 1) * 16;
             auto query = [&](int i, uint32_t(&f)[2 * NT]) { ldmatrix_x4(q_at + i * 32, f); };
             while (true) {
                 if (!mbar_wait(full + 8 * stage, phase, abort_flag, c.status, FCS_STATUS_WAIT_CONSUMER)) {
@@ -673,7 +672,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
             }
         }
 
-        // ---- the quarters of a group meet in the memory of the tiles, which all have been read
+        // ---- the warps meet in the memory of the tiles, which all have been read
         if (*abort_flag) __nanosleep(100000);      // (copies of a CTA that gave up may still be landing)
         __syncthreads();
         constexpr int PITCH = DP + 4;
@@ -682,7 +681,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
         float* part_l = part_m + 4 * SHARED_COLS;
         static_assert(4 * SHARED_COLS * (PITCH + 2) * 4 <= STAGES * L::STAGE, "the parts fit the tiles' memory");
         if (warp < SHARED_WARPS) {
-            const int at = (warp & 3) * SHARED_COLS + (warp >> 2) * NT * 8;
+            const int at = warp * SHARED_COLS;
             have.template put<PITCH>(part_o + at * PITCH, part_m + at, part_l + at);
         }
         if constexpr (CL > 1) cluster_sync(); else __syncthreads();

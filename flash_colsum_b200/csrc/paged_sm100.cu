@@ -190,7 +190,6 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
         p.cos = r->cos;
         p.sin = r->sin;
         p.rotary = r->rotary;
-        p.interleaved = r->interleaved != 0;
         p.table_rows = r->table_rows;
         p.positions = r->positions;
     }
@@ -227,7 +226,7 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
         return fail(FCS_ERR_UNSUPPORTED, "the call is too large for one launch (%lld tokens, %d heads)", T, p.q_heads);
     p.groups = (int)groups;
     const dim3 grid((unsigned)(segments * groups));
-    const int rot = !p.cos ? 0 : p.interleaved ? 2 : 1;
+    const int rot = !p.cos ? 0 : r->interleaved ? 2 : 1;
     const cudaError_t e = cache->dtype == FCS_DTYPE_BF16 ? launch_append<Bf16Ops>(rot, grid, stream, p)
                                                          : launch_append<HalfOps>(rot, grid, stream, p);
     if (e != cudaSuccess) return fail(FCS_ERR_CUDA, "appending failed to launch: %s", cudaGetErrorString(e));
@@ -455,7 +454,7 @@ struct AttendPlan {
 static AttendPlan attend_plan(const FcsPagedCache* cache, int group, int k) {
     AttendPlan a;
     const long long T = cache->tokens, B = cache->sequences;
-    a.tile_tokens = SHARED_COLS / group < 31 ? SHARED_COLS / group : 31;
+    a.tile_tokens = SHARED_COLS / group;
     const long long blocks = (a.tile_tokens > 0 && T / a.tile_tokens > B ? T / a.tile_tokens : B) * cache->kv_heads;
     const long long together = T / B < a.tile_tokens ? T / B : a.tile_tokens;
     a.shared = cache->starts && T > 2 * B && a.tile_tokens >= 2 && cache->table_width <= SHARED_PAGES &&
