@@ -59,11 +59,19 @@ int fcs_run_call(const FcsCall* call);
 int fcs_run_host_call(const FcsHostCall* call);
 }
 
-// Whether the rows of a result, `dim` elements at these strides on two axes of `size` entries each, have no element in common, so
-// that each has one writer: the shorter stride holds a row, the longer one all rows of the shorter.  (The stride of an axis of one
-// entry says nothing.)
-inline bool fcs_rows_apart(const int64_t (&size)[2], const int64_t* stride, int64_t dim) {
-    if (size[0] <= 1 || size[1] <= 1) return (size[0] <= 1 || stride[0] >= dim) && (size[1] <= 1 || stride[1] >= dim);
-    const int inner = stride[1] <= stride[0] ? 1 : 0;
-    return stride[inner] >= dim && (stride[1 - inner] - dim) / stride[inner] >= size[inner] - 1;
+// Whether rows of `dim` elements at these strides, on `n` (up to three) axes of `size` entries each, have no element in common, so that
+// each has one writer: every stride holds what the shorter ones span.  (The stride of an axis of one entry says nothing.)
+inline bool fcs_rows_apart(int n, const int64_t* size, const int64_t* stride, int64_t dim) {
+    __int128 span = dim;
+    unsigned done = 0;
+    for (int step = 0; step < n; ++step) {
+        int next = -1;
+        for (int i = 0; i < n; ++i)
+            if (!(done >> i & 1u) && (next < 0 || stride[i] < stride[next])) next = i;
+        done |= 1u << next;
+        if (size[next] <= 1) continue;
+        if (stride[next] < span) return false;
+        span += (__int128)stride[next] * (size[next] - 1);
+    }
+    return true;
 }

@@ -28,7 +28,14 @@ static int check_rows(const char* name, const void* ptr, const int64_t* stride, 
 
 static int check_result(const char* name, const FcsPagedCache* c, int q_heads, const int64_t* stride) {
     const int64_t size[2] = {c->tokens, q_heads};
-    if (fcs_rows_apart(size, stride, c->dim)) return FCS_OK;
+    if (fcs_rows_apart(2, size, stride, c->dim)) return FCS_OK;
+    return fail(FCS_ERR_INVALID_ARGUMENT, "%s strides must keep its rows apart", name);
+}
+
+// A pool that is written.
+static int check_written(const char* name, const FcsPagedCache* c, const int64_t* stride) {
+    const int64_t size[3] = {c->pages, c->kv_heads, c->page_size};
+    if (fcs_rows_apart(3, size, stride, c->dim)) return FCS_OK;
     return fail(FCS_ERR_INVALID_ARGUMENT, "%s strides must keep its rows apart", name);
 }
 
@@ -173,6 +180,8 @@ static int append(const FcsPagedCache* cache, const FcsPagedRows* r, int* status
     if ((rc = check_rows("value", r->value, r->value_stride, 2)) != FCS_OK) return rc;
     if ((rc = check_rows("key_pages", cache->key_pages, cache->key_stride, 3)) != FCS_OK) return rc;
     if ((rc = check_rows("value_pages", cache->value_pages, cache->value_stride, 3)) != FCS_OK) return rc;
+    if ((rc = check_written("key_pages", cache, cache->key_stride)) != FCS_OK) return rc;
+    if ((rc = check_written("value_pages", cache, cache->value_stride)) != FCS_OK) return rc;
     const bool with_query = r->query != nullptr;
     if (with_query) {
         if ((rc = check_rows("query", r->query, r->query_stride, 2)) != FCS_OK) return rc;

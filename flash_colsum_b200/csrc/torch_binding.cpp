@@ -381,12 +381,12 @@ bool rows_ready(const at::Tensor& t, int64_t (&st)[N]) {
 // A result of rows as the kernels write it.
 bool result_ready(const at::Tensor& t, int64_t (&st)[2]) {
     const int64_t size[2] = {t.size(0), t.size(1)};
-    return rows_ready<2>(t, st) && fcs_rows_apart(size, st, t.size(2));
+    return rows_ready<2>(t, st) && fcs_rows_apart(2, size, st, t.size(2));
 }
 
-// A pool as the kernels take it: positive strides, no two entries in one place as far as the strides say.
-bool pool_ready(const at::Tensor& t, int64_t (&st)[3]) {
-    if (!rows_ready<3>(t, st)) return false;
+// A pool as the kernels take it: strides that hold a row and, where it is written, keep the rows apart.
+bool pool_ready(const at::Tensor& t, int64_t (&st)[3], bool write) {
+    if (!rows_ready<3>(t, st) || (write && !fcs_rows_apart(3, t.sizes().data(), st, t.size(3)))) return false;
     for (int i = 0; i < 3; ++i)
         if (t.size(i) > 1 && st[i] < t.size(3)) return false;
     return true;
@@ -433,13 +433,13 @@ struct PagedArgs {
         c.tokens = (int)T;
         return true;
     }
-    bool pools(const at::Tensor& rows, const at::Tensor& k, const at::Tensor& v) {
+    bool pools(const at::Tensor& rows, const at::Tensor& k, const at::Tensor& v, bool write) {
         if (k.dim() != 4 || v.dim() != 4 || k.sizes() != v.sizes() || k.device() != dev || v.device() != dev) return false;
         if (k.scalar_type() != rows.scalar_type() || v.scalar_type() != rows.scalar_type()) return false;
         const auto n = k.sizes();
         if (n[0] < 1 || n[0] > 0x7fffffffLL || n[1] < 1 || n[1] > 65535 || n[3] != c.dim) return false;
         if (n[2] != 16 && n[2] != 32 && n[2] != 64 && n[2] != 128) return false;
-        if (!pool_ready(k, c.key_stride) || !pool_ready(v, c.value_stride)) return false;
+        if (!pool_ready(k, c.key_stride, write) || !pool_ready(v, c.value_stride, write)) return false;
         c.key_pages = const_cast<void*>(k.const_data_ptr());      // (to be read; append_paged asks again)
         c.value_pages = const_cast<void*>(v.const_data_ptr());
         c.pages = (int)n[0];
@@ -489,7 +489,7 @@ PyObject* py_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {
         const c10::OptionalDeviceGuard guard(key.is_cuda() ? std::optional<c10::Device>(key.device()) : std::nullopt);
         if (!a.batch(key, THPVariable_Unpack(args[4]), THPVariable_Unpack(args[5]), starts)) Py_RETURN_NONE;
-        if (!a.pools(key, THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]))) Py_RETURN_NONE;
+        if (!a.pools(key, THPVariable_Unpack(args[2]), THPVariable_Unpack(args[3]), true)) Py_RETURN_NONE;
         if (!like_rows(value, key) || key.size(1) != a.c.kv_heads || value.size(1) != a.c.kv_heads) Py_RETURN_NONE;
         if ((cos == nullptr) != (sin == nullptr) || (positions && !cos)) Py_RETURN_NONE;
         if (cos) {
@@ -619,7 +619,7 @@ PyObject* py_attend_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {
         const c10::OptionalDeviceGuard guard(query.is_cuda() ? std::optional<c10::Device>(query.device()) : std::nullopt);
         if (!a.batch(query, THPVariable_Unpack(args[3]), THPVariable_Unpack(args[4]), starts)) Py_RETURN_NONE;
-        if (!a.pools(query, THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2])) || !a.heads_ok(query)) Py_RETURN_NONE;
+        if (!a.pools(query, THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]), false) || !a.heads_ok(query)) Py_RETURN_NONE;
         if (!indices_ok(chosen, 3, a.dev) || chosen.size(0) != query.size(0) || chosen.size(1) != a.c.kv_heads ||
             chosen.size(2) > FCS_LIST_MAX)
             Py_RETURN_NONE;

@@ -58,11 +58,19 @@ def _check_rows(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"head_dim must be a multiple of 8 from 8 to 128, got {t.shape[2]}")
 
 
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether no row has an element in common with another: every stride holds what the shorter ones span."""
+    span = t.shape[-1]
+    for s, n in sorted(zip(t.stride()[:-1], t.shape[:-1])):
+        if n > 1:
+            if s < span:
+                return False
+            span += s * (n - 1)
+    return True
+
+
 def _check_result(name: str, t: torch.Tensor) -> None:
-    """Memory for a result: rows that can be written in pieces of 16 bytes, none of which lies in another."""
-    rows = sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1)
-    apart = all(s >= t.shape[2] for s, _ in rows) and (len(rows) < 2 or rows[1][0] >= rows[0][0] * (rows[0][1] - 1) + t.shape[2])
-    if not _rows_ready(t) or not apart:
+    if not _rows_ready(t) or not _rows_apart(t):
         raise ValueError(f"{name} needs unit inner stride, other strides in multiples of 8 elements that keep its rows apart, and a "
                          f"16-byte aligned base, got strides {t.stride()}")
 
@@ -96,7 +104,7 @@ def _check_batch(rows: torch.Tensor, page_table: torch.Tensor, lens: torch.Tenso
         raise ValueError("there are tokens and no sequence")
 
 
-def _check_pools(rows: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor) -> None:
+def _check_pools(rows: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, written: bool) -> None:
     if key_pages.ndim != 4 or key_pages.shape != value_pages.shape:
         raise ValueError(f"key_pages and value_pages must be (pages, kv_heads, page_size, head_dim) of one shape, got "
                          f"{tuple(key_pages.shape)} and {tuple(value_pages.shape)}")
@@ -110,7 +118,7 @@ def _check_pools(rows: torch.Tensor, key_pages: torch.Tensor, value_pages: torch
     for name, t in (("key_pages", key_pages), ("value_pages", value_pages)):
         if t.dtype != rows.dtype or t.device != rows.device:
             raise ValueError(f"{name} must be {rows.dtype} on {rows.device}, got {t.dtype} on {t.device}")
-        if not _rows_ready(t) or any(s < D for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+        if not _rows_ready(t) or any(s < D for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1) or (written and not _rows_apart(t)):
             raise ValueError(f"{name} needs unit inner stride, other strides in multiples of 8 elements that keep its rows "
                              f"apart, and a 16-byte aligned base, got strides {t.stride()}")
 
@@ -173,7 +181,7 @@ def append_paged(
     _check_rows("key", key)
     _check_like("value", value, key, key.shape)
     _check_batch(key, page_table, lens, starts)
-    _check_pools(key, key_pages, value_pages)
+    _check_pools(key, key_pages, value_pages, True)
     N, H, _, D = key_pages.shape
     if key.shape[1] != H:
         raise ValueError(f"the pools hold {H} heads, key has {key.shape[1]}")
@@ -314,7 +322,7 @@ def attend_pages(
             return res
     _check_rows("query", query)
     _check_batch(query, page_table, lens, starts)
-    _check_pools(query, key_pages, value_pages)
+    _check_pools(query, key_pages, value_pages, False)
     _check_heads("query", query.shape[1], key_pages.shape[1])
     _check_indices("pages", pages, query, 3)
     if tuple(pages.shape[:2]) != (query.shape[0], key_pages.shape[1]) or pages.shape[2] == 0:

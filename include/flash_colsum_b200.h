@@ -340,13 +340,14 @@ int fcs_select_threshold(const float *colsum, int64_t ld, int B, int S, float th
  * ones included, so that row t of sequence b has position lens[b] - starts[b+1] + t (lens[b] - 1
  * without starts).  Rows from starts[sequences] on belong to nobody: inputs are not read there, and
  * outputs are left as they are, or set (rotated queries and results 0, pages -1) when fill_tail is 1.
- * The rows of a result do not overlap: of its two strides the shorter holds a row, the longer all rows
- * of the shorter (an axis of one entry has none).
+ * The rows of a result do not overlap either: of its two strides the shorter holds a row, the longer all
+ * rows of the shorter (an axis of one entry has none).
  * Position i of sequence b lies in page page_table[b * table_stride + i / page_size], slot
  * i % page_size.  starts ascends, starts[0] is 0; page_table, lens and starts are device memory.
  *
  * The pools are (pages, kv_heads, page_size, dim) tensors of 16-bit elements with unit inner stride;
- * the strides of page, head and slot are multiples of 8, in any order.  page_size is 16, 32, 64 or
+ * the strides of page, head and slot are multiples of 8, in any order (for fcs_append_paged each of them holds what
+ * the shorter ones span).  page_size is 16, 32, 64 or
  * 128, dim a multiple of 8 up to 128.  The heads of a query share the keys of head / group, group =
  * q_heads / kv_heads.
  *

@@ -60,3 +60,12 @@ def test_plans_of_calls_over_a_paged_cache():
             _cabi.paged_plan(c, heads, k)
     with pytest.raises(RuntimeError, match="page size"):
         _cabi.paged_plan(cache(page_size=8), 8, 1)
+
+
+@pytest.mark.parametrize("stride", [(128, 128, 128), (0, 8192, 128), (16384, 0, 128), (16384, 8192, 0), (16384, 8192, 120), (16384, 8184, 128),
+                                    (16376, 8192, 128), (16384, 128, 248), (128, 1280, 2552)])
+def test_pools_whose_rows_overlap_are_not_written(stride):
+    """Ten pages of two heads of 64 slots of 128 features."""
+    for name in ("key", "value"):
+        assert append(cache(**{name + "_stride": stride})) < 0
+        assert f"{name}_pages strides must keep its rows apart" in _cabi.last_error()

@@ -75,6 +75,12 @@ def test_attention_over_the_longest_list(tokens):
 
 
 # --------------------------------------------------------------------------- memory for results
+def a_step(seed):
+    a = Batch(seed, [3], [40], 16, 2, 4, 64, BF16)
+    q, k, v, kp, vp, table, lens, starts = on_gpu(a.rows(4), a.rows(2), a.rows(2), a.pool(), a.pool(), a.table, a.lens, a.starts)
+    return q, k, v, kp, vp, torch.stack([kp.amin(2), kp.amax(2)], 2), table, lens, starts
+
+
 def test_results_in_memory_that_overlaps_are_refused():
     import flash_colsum_b200 as fc
     T, H, heads, D = 5, 2, 4, 64
@@ -89,6 +95,29 @@ def test_results_in_memory_that_overlaps_are_refused():
         with pytest.raises(ValueError, match="out needs .* keep its rows apart"):
             fc.attend_pages(q, kp, vp, table, lens, pages, starts=starts, out=odd)
     assert (memory == 0).all()
+    status_is(0)
+
+
+def test_pools_whose_rows_overlap_are_not_written():
+    import flash_colsum_b200 as fc
+    q, k, v, kp, vp, bounds, table, lens, starts = a_step(42)
+    memory, (N, H, P, D) = torch.zeros(kp.numel(), dtype=BF16, device="cuda"), kp.shape
+    for stride in ((D, D, D), (H * P * D, P * D, D - 8), (H * P * D, P * D - 8, D), (H * P * D - 8, P * D, D), (D, N * D, N * H * D - 8)):
+        odd = memory.as_strided(kp.shape, (*stride, 1))
+        for pools in ((odd, vp), (kp, odd)):
+            with pytest.raises(ValueError, match="keep its rows apart"):
+                fc.append_paged(k, v, *pools, table, lens, starts=starts)
+    assert (memory == 0).all()
+    want = fc.append_paged(k, v, kp, vp, table, lens, starts=starts, query=q, bounds=bounds)
+    for order in ((0, 1, 2), (0, 2, 1), (2, 1, 0), (1, 0, 2), (2, 0, 1), (1, 2, 0)):      # the axes, outermost first
+        some = [torch.zeros([kp.shape[i] + (n == 1) for n, i in enumerate(order)] + [D + 8], dtype=BF16, device="cuda")[:, :kp.shape[order[1]], :, :D]
+                .permute(*(order.index(i) for i in range(3)), 3) for _ in range(2)]
+        assert some[0].shape == kp.shape and some[0].stride() != kp.stride()
+        assert torch.equal(fc.append_paged(k, v, *some, table, lens, starts=starts, query=q), want)
+        for held, full in zip(some, (kp, vp)):
+            for i in range(40 - 3, 40):
+                page = int(table[0, i // P])
+                assert torch.equal(held[page, :, i % P], full[page, :, i % P])
     status_is(0)
 
 
@@ -110,12 +139,6 @@ def test_results_in_any_memory_that_does_not():
             assert torch.equal(odd, turned)
             assert torch.equal(fc.attend_pages(odd, kp, vp, table, lens, pages, starts=starts, out=odd), want)
     status_is(0)
-
-
-def a_step(seed):
-    a = Batch(seed, [3], [40], 16, 2, 4, 64, BF16)
-    q, k, v, kp, vp, table, lens, starts = on_gpu(a.rows(4), a.rows(2), a.rows(2), a.pool(), a.pool(), a.table, a.lens, a.starts)
-    return q, k, v, kp, vp, torch.stack([kp.amin(2), kp.amax(2)], 2), table, lens, starts
 
 
 def test_pools_that_share_their_memory_until_they_are_written():
