@@ -323,3 +323,27 @@ def test_an_attention_whose_pages_never_come_returns(tokens, H, k, twice, D):
     again = fc.attend_pages(query, kp, vp, table, lens, pages, starts=starts, return_lse=True)
     assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
     status_is(0)
+
+
+# --------------------------------------------------------------------------- bounds
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,H", [(64, 2), (128, 9)])
+def test_bounds_of_a_page_whose_slot_0_is_left_out(D, H, interleaved):
+    """A token whose position the rotation lacks is not written: where it is the first of a page, the page keeps what it had."""
+    import flash_colsum_b200 as fc
+    T, P = 48, 16
+    a = Batch(43, [T], [T], P, H, H, D, BF16)
+    key, pools = a.rows(H), [a.pool(), a.pool()]
+    bounds = torch.stack([pools[0].amin(2), pools[0].amax(2)], 2)
+    cos, sin = torch.ones(100, D // 2), torch.zeros(100, D // 2)              # (rotated by nothing: keys are stored as they are)
+    positions = torch.arange(T, dtype=torch.int32)
+    positions[16], positions[32:], positions[3] = 100, -1, -7                 # a page's first token, a page's tokens, one further in
+    d = on_gpu(key, key, *pools, a.table, a.lens, a.starts, cos, sin, positions, bounds)
+    fc.append_paged(*d[:6], starts=d[6], cos=d[7], sin=d[8], positions=d[9], bounds=d[10], interleaved=interleaved)
+    status_is(6)
+    want = bounds.clone()
+    written = key[[i for i in range(16) if i != 3]], key[17:32]
+    at = a.table[0].tolist()
+    want[at[0]] = torch.stack([written[0].amin(0), written[0].amax(0)], 1)
+    want[at[1]] = torch.stack([torch.minimum(written[1].amin(0), bounds[at[1], :, 0]), torch.maximum(written[1].amax(0), bounds[at[1], :, 1])], 1)
+    assert torch.equal(d[10].cpu(), want)
