@@ -62,6 +62,11 @@ int fcs_run_host_call(const FcsHostCall* call);
 // Whether rows of `dim` elements at these strides, on `n` (up to three) axes of `size` entries each, have no element in common, so that
 // each has one writer: every stride holds what the shorter ones span.  (The stride of an axis of one entry says nothing.)
 inline bool fcs_rows_apart(int n, const int64_t* size, const int64_t* stride, int64_t dim) {
+    // the usual order first: a stride that holds all of the axis inside it
+    int64_t held = dim;
+    int axis = n - 1;
+    while (axis >= 0 && (size[axis] <= 1 || (stride[axis] >= held && !__builtin_mul_overflow(stride[axis], size[axis], &held)))) --axis;
+    if (axis < 0) return true;
     __int128 span = dim;
     unsigned done = 0;
     for (int step = 0; step < n; ++step) {
