@@ -45,7 +45,7 @@ struct AttendParams {
     int tile_tokens;               // (attend_shared_kernel) tokens of a CTA
     float c_log2;                  // scale * log2(e)
     int fill_tail;                 // rows behind the last sequence: 1 zeros the output's, 2 sets the sums' to -inf
-    int withhold;                  // (self-test) the producer issues nothing
+    int withhold;                  // 1 (self-test): an arrival that never comes is counted, so that no wait for a tile ends
 };
 
 template <int DP, int STAGES>
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
         prefetch_tensormap(&key_map);
         prefetch_tensormap(&value_map);
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(full + 8 * s, 1);
+            mbar_init(full + 8 * s, 1 + p.withhold);
             mbar_init(empty + 8 * s, ATTEND_WARPS);
         }
         *abort_flag = 0;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
         const int e1 = min(p.k, (int)((long long)units * (rank + 1) / CL) * per_tile);
         const int* list = p.chosen + ((long long)t * c.kv_heads + h) * p.k;
         int stage = 0, phase = 1, place = 0;
-        bool fine = !p.withhold;
+        bool fine = true;
         const uint32_t piece = (uint32_t)place_keys * 128u;
         for (int base = e0; base < e1 && fine; base += 32) {
             const int e = base + lane;
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
         prefetch_tensormap(&key_map);
         prefetch_tensormap(&value_map);
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(full + 8 * s, 1);
+            mbar_init(full + 8 * s, 1 + p.withhold);
             mbar_init(empty + 8 * s, SHARED_WARPS);
         }
         flags[0] = flags[1] = flags[2] = 0;
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(SHARED_THREADS, SHARED_CTAS<DP>)
 
     // The ring goes on from pass to pass: one over the sets, and if need be one over each token's own list.
     int stage = 0, phase = warp == SHARED_WARPS ? 1 : 0;
-    bool fine = warp < SHARED_WARPS || !p.withhold;
+    bool fine = true;
     int pass = twice ? 0 : -1;
     while (true) {
         Columns<KS, NT, BF16> have;

@@ -45,7 +45,7 @@ struct SelectParams {
     int pitch, splits;
     int t0, t1;                     // tokens of this launch
     int fill_tail;
-    int withhold;                   // (self-test) no bounds are asked for
+    int withhold;                   // 1 (self-test): an arrival that never comes is counted, so that no wait for bounds ends
 };
 
 template <bool BF16>
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     __shared__ uint32_t room[2 * 3 * WARPS];
     __shared__ CloseList close;
     __shared__ __align__(16) uint16_t parts[4][2 * DP];       // what 16 bits hold, the rest of that and the rest's, zeros
-    if (threadIdx.x % 32 == 0) mbar_init(smem_u32(&arrived[threadIdx.x / 32]), 1);
+    if (threadIdx.x % 32 == 0) mbar_init(smem_u32(&arrived[threadIdx.x / 32]), 1 + p.withhold);
     if (threadIdx.x == 0) abort_flag = 0;
     mbar_fence_init();
     if constexpr (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) select_row_kernel(const
     // This warp's next 16 pages; whether each is one of the pools'.  (For one that is not, page 0 stands in.)
     auto ask = [&](int first, int entry) {
         const int n = min(16, end - first);
-        if (n <= 0 || p.withhold) return;
+        if (n <= 0) return;
         if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * 4 * D));
         __syncwarp();
         if (lane < n) {

@@ -504,10 +504,11 @@ int fcs_selftest_wait_expiry(const void *q, const void *k, void *workspace, size
 int fcs_selftest_wait_expiry_cluster(const void *q, const void *k, float *out, int *status, double limit_seconds,
                                      void *stream);
 /*
- * The same for the kernels over a paged cache: fcs_select_pages and fcs_attend_pages (which kernel, and over
- * how many CTAs, goes by the sizes as it does there) whose copies are not issued.  *status, which must not be NULL, is
- * FCS_STATUS_WAIT_CONSUMER afterwards; a row that had something to wait for chooses any pages of its sequence,
- * or gets zeros and a log-sum of -inf.  A selection of many tokens a sequence has no waits: FCS_ERR_UNSUPPORTED.
+ * The same for the kernels over a paged cache: fcs_select_pages and fcs_attend_pages (which kernel, and over how many
+ * CTAs, goes by the sizes as it does there) whose barriers count an arrival that never comes: the copies land, but no
+ * wait for them ends.  *status, which must not be NULL, is FCS_STATUS_WAIT_PRODUCER or FCS_STATUS_WAIT_CONSUMER afterwards; a
+ * row that had something to wait for chooses any pages of its sequence, or gets zeros and a log-sum of -inf.  A selection of
+ * many tokens a sequence has no waits: FCS_ERR_UNSUPPORTED.
  */
 int fcs_selftest_wait_expiry_select(const FcsPagedCache *cache, const void *query, const int64_t *query_stride,
                                     int q_heads, const void *bounds, int k, int first, int last, int *chosen,

@@ -271,7 +271,7 @@ def test_tokens_in_front_of_a_sequence_see_nothing(tokens, length):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("rows,pages,H", [(1, 40, 2), (2, 1100, 1), (150, 70, 8)])     # one CTA a row, sixteen, and one with others beside it
 def test_a_selection_whose_bounds_never_come_returns(rows, pages, H, D):
-    """No copy is issued and the limit is 50 ms: the waits run out, every CTA returns, the status word says so, what is written are
+    """The barriers count an arrival that never comes and the limit is 50 ms: the waits run out, every CTA returns, the status word says so, what is written are
     pages of the sequences; and the same call chooses as before."""
     from flash_colsum_b200 import _cabi
     lib, k = _cabi.load(), 9
@@ -288,7 +288,7 @@ def test_a_selection_whose_bounds_never_come_returns(rows, pages, H, D):
     assert lib.fcs_selftest_wait_expiry_select(ctypes.byref(c), q.data_ptr(), stride, H, b.data_ptr(), k, 1, 1, out.data_ptr(), room.data_ptr(),
                                                room.numel(), word.data_ptr(), 0.05, torch.cuda.current_stream().cuda_stream) == 0, _cabi.last_error()
     torch.cuda.synchronize()
-    assert int(word) == 3                        # FCS_STATUS_WAIT_CONSUMER
+    assert int(word) == 3                        # FCS_STATUS_WAIT_CONSUMER: a warp waits for what it asked for itself
     assert int(out.amin()) >= -1 and int(out.amax()) < pages
     assert (around[:256] == 7).all() and (around[-256:] == 7).all()
     assert torch.equal(select(a, query, bounds, k, 1, 1), first)
@@ -318,7 +318,7 @@ def test_an_attention_whose_pages_never_come_returns(tokens, H, k, twice, D):
     assert lib.fcs_selftest_wait_expiry_attend(ctypes.byref(c), query.data_ptr(), stride, H, pages.data_ptr(), k, 0.1, out.data_ptr(), stride,
                                                lse.data_ptr(), word.data_ptr(), 0.05, torch.cuda.current_stream().cuda_stream) == 0, _cabi.last_error()
     torch.cuda.synchronize()
-    assert int(word) == 3
+    assert int(word) in (1, 3)                   # (the producer waits for tiles to become free)
     assert (out == 0).all() and (lse == -torch.inf).all()
     again = fc.attend_pages(query, kp, vp, table, lens, pages, starts=starts, return_lse=True)
     assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
