@@ -456,7 +456,8 @@ __global__ void __launch_bounds__(ATTEND_THREADS)
 // count: 512 tokens that choose 32 of 512 pages each, half of them in common with their neighbours, groups of four heads: a token
 // at a time 284 us and 4.3 GB through L2; 16 columns, four tokens, 2.2 GB and 190 us with three CTAs per SM (two stages of tiles),
 // 210 us with two (three stages); 32 columns 240 us and 48 or 64 columns 230 and 236 us, one CTA per SM.  57 tokens in threes, 64
-// pages of 16 keys, heads of 64: 74 us, with four CTAs per SM 55.
+// pages of 16 keys, heads of 64: a token at a time 78 us, in blocks with four CTAs per SM 49.  The table of token sets takes shared
+// memory by its width: at heads of 128 three CTAs per SM up to about 1440 pages, two past that (the 512 tokens 225 us).
 constexpr int SHARED_NT = 2;
 constexpr int SHARED_COLS = SHARED_NT * 8;
 constexpr int SHARED_WARPS = 4;                        // consumers

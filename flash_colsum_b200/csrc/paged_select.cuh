@@ -15,8 +15,8 @@
 // chooses.  Many (score_tiles_kernel, choose_kernel): 64 tokens by 64 pages at a time, n and p in two 16-bit pieces each, and a
 // warp or a block per row chooses from the scores.
 //
-// Measured, groups of four heads of 128, pages of 64: one query, 2048 pages (8.4 MB) 11 us, a chain of loads and barriers; 32
-// sequences x 256 to 512 pages (52 MB) 23 us, 13 of them while the bounds come at 4 TB/s, 5 of choosing behind them; 1021 tokens x
+// Measured, groups of four heads of 128, pages of 64: one query, 2048 pages (8.4 MB) 11 us, a chain of loads and barriers, 7 of them
+// without choosing; 32 sequences x 256 to 512 pages (52 MB) in clusters of two 23 us, 17 of them without choosing; 1021 tokens x
 // 512 pages 54 us, 27 of scores (matrix pipe 30 % busy) and 27 of choosing (2100 instructions a row, issue slots 64 % busy).
 // With 64-bit sums throughout these were 26, 42 and 1022 us.
 #pragma once
@@ -578,7 +578,9 @@ __device__ __forceinline__ bool settled(const SelectParams& p, int b, const Row&
 
 // ------------------------------------------------------------------ few tokens a sequence
 constexpr int ROW_THREADS = 128;
-constexpr int ROW_CTAS = 6;          // per SM (three of 256 threads: 32 sequences 23.4 us for 23.2)
+// Per SM, by the registers (three of 256 threads take as long, within what two runs differ by).  Shared memory has a score for every
+// page of the table's width: at heads of 128 it holds six CTAs up to 350 pages, five at 512, four at 4096, three at 8192.
+constexpr int ROW_CTAS = 6;
 typedef BlockTeam<ROW_THREADS, 16> RowTeam;
 
 // grid: (CL * tokens, kv heads); shared memory: row_smem.  A warp takes 16 pages at a time, whose bounds bulk copies bring -- it

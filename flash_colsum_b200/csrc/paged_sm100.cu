@@ -459,7 +459,9 @@ struct AttendPlan {
 // Tokens of a sequence share what they chose in common, where there are enough of them: more than two a sequence, and blocks
 // for all SMs or of eight tokens.  Measured, blocks against a token at a time, 32 pages of 64 for groups of four heads: 512
 // blocks of two tokens 127 and 121 us; 256 of four 96 and 105, 192 of four 50 and 62; 128 of four 48 and 42 (58 and 52), 64
-// of four 34 and 22; heads of their own, 64 of sixteen 53 and 60, 32 of sixteen 29 and 39.
+// of four 34 and 22; heads of their own, 64 of sixteen 53 and 60, 32 of sixteen 29 and 39.  512 tokens of eight key/value heads in
+// groups of one 118 and 271, two 151 and 275, four 191 and 283, five (three tokens a block) 221 and 285, eight (two) 245 and 296;
+// of four in groups of eight 142 and 148.
 static AttendPlan attend_plan(const FcsPagedCache* cache, int group, int k) {
     AttendPlan a;
     const long long T = cache->tokens, B = cache->sequences;
